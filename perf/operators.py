@@ -1,0 +1,265 @@
+"""Cases for timing the optimizer-side operators (global gradient norm, clipping by it, the Adam update that clips on the way)
+and the 8-bit integer products of the regressor's fully connected head, beside their plain forms in torch operations.
+
+`own` False: `run` computes with elementary torch operations.  `own` True: `run` makes the calls of the package's `ops`."""
+import math
+import random
+
+import torch
+
+own = False
+
+DTYPES = {'float32': torch.float32, 'bfloat16': torch.bfloat16, 'float16': torch.float16}
+SIZE = {'float32': 4, 'bfloat16': 2, 'float16': 2}
+LR, BETA1, BETA2 = 1e-4, 0.9, 0.999
+STEP = 100                                           # Adam's t: an early step, where the bias corrections still matter
+EPS = 1e-8 / math.sqrt(1.0 - BETA2 ** STEP)          # the trainer's rule (epsilon-hat form) at that step
+
+
+# ---- shapes -----------------------------------------------------------------------------------------------------------
+def regressor_shapes(patch):
+    """The 20 variables of the regressor at patch size `patch`: eight 3x3 convolutions, fc1 and fc2, each weight and bias."""
+    chans = [(2, 64), (64, 64), (64, 64), (64, 64), (64, 128), (128, 128), (128, 128), (128, 128)]
+    shapes = []
+    for i, o in chans:
+        shapes += [(o, i, 3, 3), (o,)]
+    feat = patch // 8
+    return shapes + [(1024, feat * feat * 128), (1024,), (8, 1024), (8,)]
+
+
+def list_shapes(case):
+    """A case's tensors: the regressor's variables, or `tensors` vectors of 1 to `largest` elements (odd ones among them)."""
+    if case['patch']:
+        return regressor_shapes(case['patch'])
+    rng = random.Random(case['tensors'] * 1000003 + case['largest'])
+    return [(int(round(math.exp(rng.uniform(0.0, math.log(case['largest']))))),) for _ in range(case['tensors'])]
+
+
+def list_dtypes(case):
+    n = len(list_shapes(case))
+    if case['dtype'] == 'mixed':
+        names = ('float32', 'bfloat16', 'float16')
+        return [names[i % 3] for i in range(n)]
+    return [case['dtype']] * n
+
+
+def padded_rows(rows, cols, device):
+    """int8 [rows, cols] as the package's row quantiser lays it out: row starts on 128 bytes."""
+    return torch.zeros((rows, -(-cols // 128) * 128), dtype=torch.int8, device=device)[:, :cols]
+
+
+# ---- cases ------------------------------------------------------------------------------------------------------------
+def grad_case(op, name, patch=0, tensors=0, largest=0, dtype='float32', clip=1.0):
+    return {'name': name, 'op': op, 'patch': patch, 'tensors': tensors, 'largest': largest, 'dtype': dtype, 'clip': clip}
+
+
+def int8_case(op, name, m, n, k, dtype='float32', bias=True, relu=True):
+    return {'name': name, 'op': op, 'm': m, 'n': n, 'k': k, 'dtype': dtype, 'bias': bias, 'relu': relu}
+
+
+def listed():
+    return [
+        # the gradient norm a training log prints: the regressor at the default patch size, 34 M float32 gradients
+        grad_case('norm', 'norm_regressor_p128', patch=128),
+        # many small tensors of several types (adapters, biases, norms of a mixed-precision model): launch latency
+        grad_case('norm', 'norm_300_small_mixed', tensors=300, largest=5000, dtype='mixed'),
+        # clipping before an optimizer that takes gradients: the regressor again
+        grad_case('clip', 'clip_regressor_p128', patch=128),
+        # ... and a short list of 16-bit gradients of odd lengths
+        grad_case('clip', 'clip_40_bf16', tensors=40, largest=60000, dtype='bfloat16'),
+        # the optimizer step of the training loop with clipping, default patch size
+        grad_case('adam', 'adam_regressor_p128', patch=128),
+        # ... and of the small networks (32 px patches), where launches count
+        grad_case('adam', 'adam_regressor_p32', patch=32),
+        # fc1 for one image pair: a single row against the whole weight (latency of an online prediction)
+        int8_case('matmul', 'matmul_fc1_one_pair', 1, 1024, 32768),
+        # fc1 at the trainer's batch, rows quantised before
+        int8_case('matmul', 'matmul_fc1_b64', 64, 1024, 32768),
+        # a large product: many rows, square weight
+        int8_case('matmul', 'matmul_4096_bf16', 4096, 4096, 8192, 'bfloat16', relu=False),
+        # the test loop's fc1 from float activations at the default batch
+        int8_case('linear', 'linear_fc1_b128', 128, 1024, 32768),
+        # ... for one pair
+        int8_case('linear', 'linear_fc1_one_pair', 1, 1024, 32768),
+        # odd sizes in every dimension, 16-bit activations
+        int8_case('linear', 'linear_odd_f16', 333, 1001, 2051, 'float16', bias=False, relu=False),
+    ]
+
+
+def log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(('norm', 'clip', 'adam', 'matmul', 'linear'))
+    if op in ('matmul', 'linear'):
+        m = 1 if rng.random() < 0.2 else log_int(rng, 2, 4096)
+        n, k = log_int(rng, 8, 4096), log_int(rng, 64, 32768)
+        m = min(m, 2 ** 37 // (n * k))                     # no more work than the largest listed product
+        c = int8_case(op, '', m, n, k, rng.choice(('float32', 'bfloat16', 'float16')), rng.random() < 0.7, rng.random() < 0.5)
+    elif rng.random() < 0.5:
+        dtype = rng.choice(('float32', 'bfloat16', 'float16'))
+        c = grad_case(op, '', patch=8 * rng.randint(2, 16), dtype=dtype, clip=rng.choice((0.5, 1.0, 10.0)))
+    else:
+        most = {'norm': 400, 'clip': 60, 'adam': 20}[op]
+        dtype = rng.choice(('float32', 'bfloat16', 'float16', 'mixed'))
+        c = grad_case(op, '', tensors=log_int(rng, 1, most), largest=log_int(rng, 2, 400000), dtype=dtype, clip=rng.choice((0.5, 1.0, 10.0)))
+    del c['name']
+    return c
+
+
+# ---- inputs -----------------------------------------------------------------------------------------------------------
+def like(t):
+    """Convolution weights and their gradients are kept channels-last, as the trainer keeps them."""
+    return t.contiguous(memory_format=torch.channels_last) if t.dim() == 4 else t
+
+
+def prepare(case, seed):
+    dev = torch.device('cuda:0')
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    normal = lambda shape: torch.randn(shape, generator=gen, device=dev)
+    state = {'case': case}
+    if case['op'] in ('norm', 'clip', 'adam'):
+        shapes, dtypes = list_shapes(case), list_dtypes(case)
+        scales = [10.0 ** random.Random(seed * 7919 + i).uniform(-3.0, -1.0) for i in range(len(shapes))]     # tensors differ by orders
+        state['grads'] = [like(normal(s) * c).to(DTYPES[d]) for s, c, d in zip(shapes, scales, dtypes)]
+        if case['op'] == 'adam':
+            state['params'] = [like(normal(s) * 0.05) for s in shapes]
+            state['exp_avgs'] = [like(normal(s) * c * 0.3) for s, c in zip(shapes, scales)]
+            state['exp_avg_sqs'] = [like((normal(s) * c).square() * 0.1) for s, c in zip(shapes, scales)]
+        return state
+    m, n, k = case['m'], case['n'], case['k']
+    state['weight'] = padded_rows(n, k, dev)
+    state['weight'].copy_(torch.randint(-127, 128, (n, k), generator=gen, device=dev, dtype=torch.int8))
+    state['weight_scale'] = (0.5 + torch.rand((n,), generator=gen, device=dev)) * (2.0 / math.sqrt(k) / 127.0)
+    state['bias'] = normal((n,)) * 0.1 if case['bias'] else None
+    if case['op'] == 'matmul':
+        state['x'] = padded_rows(m, k, dev)
+        state['x'].copy_(torch.randint(-127, 128, (m, k), generator=gen, device=dev, dtype=torch.int8))
+        state['x_scale'] = (0.5 + torch.rand((m,), generator=gen, device=dev)) / 127.0
+    else:                                                  # what the last convolution leaves: rectified values, rows of unlike size
+        state['x'] = (normal((m, k)).relu() * (0.2 + torch.rand((m, 1), generator=gen, device=dev))).to(DTYPES[case['dtype']])
+    return state
+
+
+# ---- plain forms --------------------------------------------------------------------------------------------------------
+def plain_norm(tensors):
+    return torch.stack([t.float().square().sum() for t in tensors]).sum().sqrt()
+
+
+def plain_clip(tensors, clip):
+    norm = plain_norm(tensors)
+    factor = clip / norm.clamp(min=clip)
+    return [(t.float() * factor).to(t.dtype) for t in tensors], norm
+
+
+def plain_adam_one(p, g, m, v, factor):
+    g = g.float() * factor
+    m.mul_(BETA1).add_(g * (1.0 - BETA1))
+    v.mul_(BETA2).add_(g.square() * (1.0 - BETA2))
+    p.sub_(LR / (1.0 - BETA1 ** STEP) * m / (v.sqrt() / math.sqrt(1.0 - BETA2 ** STEP) + EPS))
+
+
+def plain_adam(params, grads, exp_avgs, exp_avg_sqs, clip):
+    norm = plain_norm(grads)
+    factor = clip / norm.clamp(min=clip)
+    [plain_adam_one(p, g, m, v, factor) for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs)]
+    return norm
+
+
+def plain_quantise(x):
+    """Rows in 8 bits: scale = max |x| / 127, values round(x * (127 / max |x|)); in 64 bits what decides on a border."""
+    top = x.abs().amax(dim=1).double()
+    inverse, scale = (127.0 / top).float(), (top / 127.0).float()
+    q = torch.round(x.double() * inverse.double()[:, None])
+    return q.float(), scale
+
+
+def plain_matmul(x, x_scale, weight, weight_scale, bias, relu, dtype):
+    y = (x.float() @ weight.float().t()) * x_scale[:, None] * weight_scale
+    y = y if bias is None else y + bias
+    y = y.relu() if relu else y
+    return y.to(dtype)
+
+
+def run(state):
+    case = state['case']
+    op = case['op']
+    if own:
+        from unsuperviseddeephomographyral2018_amd import ops
+        if op == 'norm':
+            return ops.global_norm(state['grads'])
+        if op == 'clip':
+            return ops.clip_by_global_norm(state['grads'], case['clip'])
+        if op == 'adam':
+            norm = ops.adam_clip_update_(state['params'], state['grads'], state['exp_avgs'], state['exp_avg_sqs'], lr=LR,
+                                         beta1=BETA1, beta2=BETA2, eps=EPS, step=STEP, clip_norm=case['clip'])
+            return state['params'], state['exp_avgs'], state['exp_avg_sqs'], norm
+        if op == 'matmul':
+            return ops.int8_matmul(state['x'], state['x_scale'], state['weight'], state['weight_scale'], bias=state['bias'],
+                                   relu=case['relu'], out_dtype=DTYPES[case['dtype']])
+        return ops.int8_linear(state['x'], state['weight'], state['weight_scale'], bias=state['bias'], relu=case['relu'])
+    if op == 'norm':
+        return plain_norm(state['grads'])
+    if op == 'clip':
+        return plain_clip(state['grads'], case['clip'])
+    if op == 'adam':
+        norm = plain_adam(state['params'], state['grads'], state['exp_avgs'], state['exp_avg_sqs'], case['clip'])
+        return state['params'], state['exp_avgs'], state['exp_avg_sqs'], norm
+    if op == 'matmul':
+        x, x_scale = state['x'], state['x_scale']
+    else:
+        x, x_scale = plain_quantise(state['x'])
+    return plain_matmul(x, x_scale, state['weight'], state['weight_scale'], state['bias'], case['relu'], DTYPES[case['dtype']])
+
+
+# ---- what a pass cannot do without --------------------------------------------------------------------------------------
+def work(case):
+    if case['op'] in ('norm', 'clip', 'adam'):
+        counts = [math.prod(s) for s in list_shapes(case)]
+        grad_bytes = sum(c * SIZE[d] for c, d in zip(counts, list_dtypes(case)))
+        total = sum(counts)
+        if case['op'] == 'norm':
+            return {'bytes': grad_bytes + 4, 'flops': 2 * total}
+        if case['op'] == 'clip':
+            return {'bytes': 2 * grad_bytes + 4, 'flops': 3 * total}
+        return {'bytes': grad_bytes + 24 * total + 4, 'flops': 16 * total}
+    m, n, k = case['m'], case['n'], case['k']
+    size = SIZE[case['dtype']]
+    rows = m * k + 4 * m if case['op'] == 'matmul' else m * k * size
+    return {'bytes': rows + n * k + 4 * n + (4 * n if case['bias'] else 0) + m * n * size, 'flops': 2 * m * n * k}
+
+
+# ---- the definitions in 64 bits -------------------------------------------------------------------------------------------
+def exact(case, seed):
+    state = prepare(case, seed)
+    if case['op'] in ('norm', 'clip', 'adam'):
+        norm = math.sqrt(sum(float(torch.linalg.vector_norm(g.double())) ** 2 for g in state['grads']))
+        told = torch.tensor(norm, dtype=torch.float64, device='cuda:0')
+        if case['op'] == 'norm':
+            return told
+        ratio = min(1.0, case['clip'] / norm)
+        if case['op'] == 'clip':
+            return [g.double() * ratio for g in state['grads']], told
+        params, firsts, seconds = [], [], []
+        for p, g, m, v in zip(state['params'], state['grads'], state['exp_avgs'], state['exp_avg_sqs']):
+            g = ratio * g.double()
+            first = BETA1 * m.double() + (1.0 - BETA1) * g
+            second = BETA2 * v.double() + (1.0 - BETA2) * g * g
+            mean, var = first / (1.0 - BETA1 ** STEP), second / (1.0 - BETA2 ** STEP)
+            params.append(p.double() - LR * mean / (torch.sqrt(var) + EPS))
+            firsts.append(first)
+            seconds.append(second)
+        return params, firsts, seconds, told
+    weight, scale = state['weight'].double(), state['weight_scale'].double()
+    if case['op'] == 'matmul':
+        rows, row_scale = state['x'].double(), state['x_scale'].double()
+    else:
+        # the two factors of a row are numbers of 32 bits: 127 / top, which the values are multiplied with, and top / 127
+        top = state['x'].abs().max(dim=1).values.double()
+        rows = torch.round(state['x'].double() * (127.0 / top).float().double().unsqueeze(1))
+        row_scale = (top / 127.0).float().double()
+    y = torch.mm(rows, weight.t().contiguous()) * torch.outer(row_scale, scale)
+    if case['bias']:
+        y = y + state['bias'].double().unsqueeze(0)
+    return torch.where(y > 0, y, torch.zeros_like(y)) if case['relu'] else y
