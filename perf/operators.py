@@ -97,13 +97,15 @@ def draw(rng):
         n, k = log_int(rng, 8, 4096), log_int(rng, 64, 32768)
         m = min(m, 2 ** 37 // (n * k))                     # no more work than the largest listed product
         c = int8_case(op, '', m, n, k, rng.choice(('float32', 'bfloat16', 'float16')), rng.random() < 0.7, rng.random() < 0.5)
-    elif rng.random() < 0.5:
-        dtype = rng.choice(('float32', 'bfloat16', 'float16'))
-        c = grad_case(op, '', patch=8 * rng.randint(2, 16), dtype=dtype, clip=rng.choice((0.5, 1.0, 10.0)))
     else:
-        most = {'norm': 400, 'clip': 60, 'adam': 20}[op]
         dtype = rng.choice(('float32', 'bfloat16', 'float16', 'mixed'))
-        c = grad_case(op, '', tensors=log_int(rng, 1, most), largest=log_int(rng, 2, 400000), dtype=dtype, clip=rng.choice((0.5, 1.0, 10.0)))
+        # gradients in float16 are kept scaled up, their clip with them: small ones would leave the type's range
+        clip = rng.choice((64.0, 512.0) if dtype in ('float16', 'mixed') else (0.5, 1.0, 10.0))
+        if rng.random() < 0.5:
+            c = grad_case(op, '', patch=8 * rng.randint(2, 16), dtype=dtype, clip=clip)
+        else:
+            most = {'norm': 400, 'clip': 60, 'adam': 20}[op]
+            c = grad_case(op, '', tensors=log_int(rng, 1, most), largest=log_int(rng, 2, 400000), dtype=dtype, clip=clip)
     del c['name']
     return c
 
