@@ -216,14 +216,10 @@ class Dataloader(object):
         os.ftruncate(fd, slots * H * W * 3)
         os.close(fd)
         frames = np.memmap(path, dtype=np.uint8, mode='r+', shape=(nbuf, 2, B, H, W, 3))
-        # page-lock the ring so that the uploads are DMA copies that run beside the training step (a pageable source is
-        # staged through a bounce buffer by the calling thread); a refusal only means slower, synchronous uploads
-        pinned = False
-        if self.device.type == 'cuda':
-            try:
-                pinned = int(torch.cuda.cudart().cudaHostRegister(frames.ctypes.data, frames.nbytes, 0)) == 0
-            except Exception:
-                pinned = False
+        # uploads go through one page-locked batch, so that they are DMA copies that run beside the training step (a pageable
+        # source is staged by the calling thread).  It is ALLOCATED page-locked: registering the ring's own memory is refused on
+        # some hosts, and the error that such a refusal leaves behind is reported by the next, unrelated GPU call
+        stage = torch.empty((2, B, H, W, 3), dtype=torch.uint8, pin_memory=True) if self.device.type == 'cuda' else None
         script = os.path.join(os.path.dirname(os.path.abspath(__file__)), '_decode_worker.py')
         K = self.num_workers
         import queue
@@ -301,11 +297,13 @@ class Dataloader(object):
                         body = ans.split(' ', 1)
                         if len(body) > 1 and body[1].startswith('!'):          # "slot !ErrorType: message"
                             raise RuntimeError('decode worker: ' + ans)
-                I8 = torch.from_numpy(frames[buf, 0]).to(self.device, non_blocking=pinned)
-                Ip8 = torch.from_numpy(frames[buf, 1]).to(self.device, non_blocking=pinned)
-                if pinned:                                       # the ring slot is free again once the DMA has read it
-                    torch.cuda.current_stream(self.device).synchronize()
-                # (pageable source: the copy has read the ring buffer when .to() returns)
+                if stage is not None:
+                    stage.copy_(torch.from_numpy(frames[buf]))
+                    I8 = stage[0].to(self.device, non_blocking=True)
+                    Ip8 = stage[1].to(self.device, non_blocking=True)
+                    torch.cuda.current_stream(self.device).synchronize()     # the next batch overwrites `stage`
+                else:
+                    I8, Ip8 = torch.from_numpy(frames[buf, 0]).clone(), torch.from_numpy(frames[buf, 1]).clone()
                 free.append(buf)
                 yield self._finish(I8, Ip8, ids)
         finally:
@@ -319,11 +317,6 @@ class Dataloader(object):
                     p.wait(timeout=5)
                 except Exception:
                     p.kill()
-            if pinned:
-                try:
-                    torch.cuda.cudart().cudaHostUnregister(frames.ctypes.data)
-                except Exception:
-                    pass
             del frames
             unlink_ring()
 
@@ -376,7 +369,7 @@ class Dataloader(object):
                 yield item
         finally:
             # closing (or dropping) this generator must END the producer: it is the producer's `finally` that stops the decode
-            # workers and releases the page-locked frame ring; a daemon thread that is merely abandoned never gets there
+            # workers and releases the frame ring; a daemon thread that is merely abandoned never gets there
             stop.set()
             try:
                 while True:                                   # a producer blocked on a full queue sees `stop` within 0.1 s;

@@ -460,7 +460,7 @@ def train(args):
                 torch.save(step_fn.state_dict(), ckpt)
     finally:
         if disk is not None:
-            disk.close()             # ends the producer thread, the decode workers and the page-locked frame ring -- also on
+            disk.close()             # ends the producer thread, the decode workers and the frame ring -- also on
                                      # an exception or Ctrl-C (the ring used to outlive the process)
     if rank == 0:
         os.makedirs(ckpt_dir, exist_ok=True)
