@@ -613,7 +613,7 @@ def main():
     tt = torch.tensor([dt], dtype=torch.float64, device=device)
     exchange = None
     if world > 1:
-        torch.distributed.all_reduce(tt, op=torch.distributed.ReduceOp.MAX)
+        uh_dist.all_reduce(tt, op=torch.distributed.ReduceOp.MAX)
         # the exchange step on its own and the step WITHOUT it (collective: every rank takes part) -- dist.exchange_report
         def run_steps(n):
             for _ in range(n):

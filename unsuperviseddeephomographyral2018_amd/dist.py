@@ -63,13 +63,43 @@ def init_from_env(backend=None):
     return rank, world, local
 
 
+class _Done(object):
+    def wait(self):
+        return True
+
+
+def _through_host(t):
+    """gloo gets host memory only: its collectives on device tensors have hung where several ranks share one GPU."""
+    return t.is_cuda and dist.get_backend() == 'gloo'
+
+
+def all_reduce(t, op=dist.ReduceOp.SUM, async_op=False):
+    """dist.all_reduce; a device tensor under gloo is exchanged through a synchronous host copy (the handle is then done)."""
+    if not _through_host(t):
+        return dist.all_reduce(t, op=op, async_op=async_op)
+    host = t.cpu().contiguous()
+    dist.all_reduce(host, op=op)
+    t.copy_(host)
+    return _Done() if async_op else None
+
+
+def broadcast(t, src=0):
+    """dist.broadcast, through a host copy where all_reduce does the same."""
+    if not _through_host(t):
+        return dist.broadcast(t, src=src)
+    host = t.cpu().contiguous()
+    dist.broadcast(host, src=src)
+    t.copy_(host)
+
+
 def self_launch(nproc, target, argv, module=False):
     """A program asked for `nproc` > 1 GPUs (bench.py --gpus N; the trainer's --num_gpus N, the reference's tower count,
     homography_CNN_synthetic.py:56,199-207) with no launcher around it (no WORLD_SIZE in the environment): become
     `python -m torch.distributed.run --nnodes=1 --nproc-per-node N --master-addr 127.0.0.1 --master-port <free> <target>
     <same arguments>` -- one rank per GPU; the ranks pick RCCL when every rank has a device of its own and gloo otherwise
     (init_from_env), so the same command is a functional run on a 1-GPU box.  `target` is a script path, or a module name
-    with module=True (torchrun's -m).  Replaces the process: does not return."""
+    with module=True (torchrun's -m).  Replaces the process, or, in one that has initialised the GPU already (such a process must
+    not exec), runs the launcher as a child and exits with its code: does not return."""
     import socket
     import sys
     with socket.socket() as so:
@@ -80,6 +110,9 @@ def self_launch(nproc, target, argv, module=False):
     cmd += (['-m', target] if module else [os.path.abspath(target)]) + list(argv)
     os.environ.setdefault('HSA_ENABLE_IPC_MODE_LEGACY', '0')
     sys.stdout.flush(); sys.stderr.flush()
+    if torch.cuda.is_initialized():
+        import subprocess
+        sys.exit(subprocess.run(cmd).returncode)
     os.execv(sys.executable, cmd)
 
 
@@ -231,7 +264,7 @@ class GradAverager(object):
         def hook(param):
             bucket['pending'] -= 1
             if bucket['pending'] == 0 and self.world > 1 and self.enabled:
-                self._handles.append(dist.all_reduce(bucket['flat'], op=self._op, async_op=True))
+                self._handles.append(all_reduce(bucket['flat'], op=self._op, async_op=True))
         return hook
 
     def reset(self):
@@ -253,7 +286,7 @@ class GradAverager(object):
             import time
             for b in self.buckets:
                 if b['pending'] != 0:          # a parameter received no gradient: reduce it now
-                    self._handles.append(dist.all_reduce(b['flat'], op=self._op, async_op=True))
+                    self._handles.append(all_reduce(b['flat'], op=self._op, async_op=True))
             t0 = time.perf_counter()
             for h in self._handles:
                 h.wait()
@@ -271,13 +304,13 @@ class GradAverager(object):
         out = []
         for b in self.buckets:
             buf = torch.empty_like(b['flat'])
-            dist.all_reduce(buf, op=self._op)                      # warm-up (communicator / buffers)
+            all_reduce(buf, op=self._op)                      # warm-up (communicator / buffers)
             if buf.is_cuda:
                 torch.cuda.synchronize(buf.device)
             dist.barrier()
             t0 = time.perf_counter()
             for _ in range(iters):
-                dist.all_reduce(buf, op=self._op)
+                all_reduce(buf, op=self._op)
             if buf.is_cuda:
                 torch.cuda.synchronize(buf.device)
             dt = (time.perf_counter() - t0) / iters
@@ -335,7 +368,7 @@ def exchange_report(averager, run_steps, ms_per_step=None, steps_without=10, buc
         run_steps(n)
         sync(); dist.barrier(); sync()
         tt = torch.tensor([time.perf_counter() - t0], dtype=torch.float64, device=dev)
-        dist.all_reduce(tt, op=dist.ReduceOp.MAX)
+        all_reduce(tt, op=dist.ReduceOp.MAX)
         return float(tt.item()) / n * 1e3
     try:
         if ms_per_step is None:                             # the caller has no like-for-like figure (a trainer whose loop also
@@ -371,7 +404,7 @@ def broadcast_state(module_and_optimizer, src=0):
     module, opt = module_and_optimizer
     n = 0
     for t in list(module.parameters()) + list(module.buffers()):
-        dist.broadcast(t.data, src=src)
+        broadcast(t.data, src=src)
         n += 1
     if opt is not None:
         for group in opt.param_groups:
@@ -382,10 +415,10 @@ def broadcast_state(module_and_optimizer, src=0):
                     if torch.is_tensor(v):
                         if v.device.type == 'cpu' and dist.get_backend() == 'nccl':      # a host-side step counter: via the device
                             tmp = v.to(p.device)
-                            dist.broadcast(tmp, src=src)
+                            broadcast(tmp, src=src)
                             v.copy_(tmp.cpu())
                         else:
-                            dist.broadcast(v, src=src)
+                            broadcast(v, src=src)
                         n += 1
     return n
 
@@ -423,7 +456,7 @@ class TowerMonitors(object):
         mon = torch.cat([self.totals, self.window, self.nonfinite.reshape(1),
                          torch.tensor([float(extra_count)], device=self.totals.device)]).double()
         if self.world > 1:
-            dist.all_reduce(mon)
+            all_reduce(mon)
             self.collectives += 1
         k = self.k
         out = {'avg': (mon[:k] / (self.world * max(self.steps, 1))).tolist(),
@@ -439,6 +472,6 @@ def all_reduce_mean_scalars(values, world):
     if world == 1:
         return values
     t = torch.stack([v.detach().float().reshape(()) for v in values])
-    dist.all_reduce(t, op=dist.ReduceOp.SUM)
+    all_reduce(t, op=dist.ReduceOp.SUM)
     t = t / world
     return [t[i] for i in range(len(values))]

@@ -154,7 +154,7 @@ class TrainStep(object):
         self.rank = torch.distributed.get_rank() if (world > 1 and torch.distributed.is_initialized()) else 0
         if world > 1:                                       # identical initial variables on every rank
             for t in list(self.net.parameters()) + list(self.net.buffers()):
-                torch.distributed.broadcast(t.data, src=0)
+                uh_dist.broadcast(t.data, src=0)
             # ... and independent dropout masks per tower, as the reference's one-dropout-op-per-tower graph draws them
             # (homography_model.py:120-121,128; SURVEY 8e "Dropout RNG per rank").  World size 1 keeps the caller's seed.
             self.model_rng_seed = uh_dist.seed_tower_rng(getattr(args, 'seed', 0), self.rank)
@@ -661,7 +661,7 @@ def main(argv=None):
         raise SystemExit('homography_CNN_synthetic: %s' % e)
     if args.mode == 'train':
         if what == 'launch':
-            if torch.cuda.is_available() and torch.cuda.device_count() < world:
+            if 0 < torch.cuda.device_count() < world:     # counting devices does not initialise the GPU: self_launch may still exec
                 print('note: --num_gpus %d with %d visible GPU(s): the ranks share the visible device(s) over gloo (a functional '
                       'run, not a scaling run)' % (world, torch.cuda.device_count()), file=sys.stderr, flush=True)
             uh_dist.self_launch(world, MODULE, argv, module=True)          # does not return
