@@ -15,8 +15,11 @@ LIBDIR = os.path.join(HERE, 'lib')
 LIB = os.path.join(LIBDIR, 'libuh_hotpath.so')
 SOURCES = ['uh_dlt.hip', 'uh_warp.hip', 'uh_misc.hip', 'uh_patch.hip', 'uh_losses.hip', 'uh_inputs.hip', 'uh_tail.hip', 'uh_epilogue.hip']
 HEADERS = ['uh_device.h', 'uh_host.h', os.path.join('..', '..', 'include', 'uh_hotpath.h')]
+# `-packed-fp32-ops`: no v_pk_{add,mul,fma}_f32 anywhere -- some of their forms have given wrong results now and then on gfx950.
+# The scalar forms round the same, and every kernel keeps its register count (the warp and patch kernels lose 224 packed
+# instructions, the others had none).  hipcc's host pass warns that it does not know the feature: harmless.
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-ffp-contract=off', '-fno-slp-vectorize', '-fPIC', '-shared',
-         '-fvisibility=hidden', '-Wall', '-Wno-unused-function']
+         '-fvisibility=hidden', '-Wall', '-Wno-unused-function', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def _fingerprint():
