@@ -66,7 +66,30 @@ SIGNATURES = {
     'uh_kernel_name': (C.c_char_p, [_i]),
 }
 
+# ---- include/uh_model_ops.h ------------------------------------------------------------------------------------------
+MODEL_OPS_PATH = os.path.join(HERE, 'lib', 'libuh_model_ops.so')
+UHM_ABI_VERSION = 1
+UHM_F32, UHM_BF16, UHM_F16 = 0, 1, 2
+UHM_SKIP_NONFINITE = 1
+UHM_RELU = 1
+_q = C.c_longlong
+_d = C.c_double
+_f = C.c_float
+
+MODEL_OPS_SIGNATURES = {
+    'uhm_abi_version': (_i, []),
+    'uhm_error_string': (C.c_char_p, [_i]),
+    'uhm_multi_workspace_bytes': (_z, [_i]),
+    'uhm_global_norm': (_i, [_p, _p, _p, _i, _p, _p, _z, _p]),
+    'uhm_clip_by_global_norm': (_i, [_p, _p, _p, _p, _i, _f, _p, _p, _p, _z, _p]),
+    'uhm_adam_clip_update': (_i, [_p] * 6 + [_i, _d, _d, _d, _d, _q, _f, _u, _p, _p, _p, _z, _p]),
+    'uhm_quantize_rows': (_i, [_p, _i, _q, _p, _q, _p, _q, _q, _p]),
+    'uhm_int8_matmul_workspace_bytes': (_z, [_q, _q, _q]),
+    'uhm_int8_matmul': (_i, [_p, _q, _p, _p, _q, _p, _p, _p, _i, _q, _q, _q, _u, _p, _z, _p]),
+}
+
 _lib = None
+_model_ops = None
 
 
 class UHError(RuntimeError):
@@ -90,6 +113,30 @@ def load():
         raise UHError('ABI version mismatch: library %d, binding %d' % (lib.uh_abi_version(), UH_ABI_VERSION))
     _lib = lib
     return lib
+
+
+def load_model_ops():
+    """Load libuh_model_ops.so (once) and type every entry point.  Raises if anything is missing."""
+    global _model_ops
+    if _model_ops is not None:
+        return _model_ops
+    if not os.path.exists(MODEL_OPS_PATH):
+        raise UHError('%s not found -- run `python -c "import __graft_entry__ as g; g.build()"` '
+                      '(hipcc --offload-arch=gfx950).  There is no CPU fallback.' % MODEL_OPS_PATH)
+    lib = C.CDLL(MODEL_OPS_PATH)
+    for name, (res, args) in MODEL_OPS_SIGNATURES.items():
+        fn = getattr(lib, name)
+        fn.restype = res
+        fn.argtypes = args
+    if lib.uhm_abi_version() != UHM_ABI_VERSION:
+        raise UHError('ABI version mismatch: library %d, binding %d' % (lib.uhm_abi_version(), UHM_ABI_VERSION))
+    _model_ops = lib
+    return lib
+
+
+def check_model(code, what):
+    if code != 0:
+        raise UHError('%s failed: %s (code %d)' % (what, load_model_ops().uhm_error_string(code).decode(), code))
 
 
 def check(code, what):

@@ -1,4 +1,5 @@
-"""Build the gfx950 C-ABI shared library IN-TREE (lib/libuh_hotpath.so).
+"""Build the gfx950 C-ABI shared libraries IN-TREE: lib/libuh_hotpath.so (include/uh_hotpath.h) and lib/libuh_model_ops.so
+(include/uh_model_ops.h).
 
 hipcc cross-compiles without a GPU.  The built .so is git-ignored but travels to the GPU box with
 the gpurun snapshot.  `-ffp-contract=off` is part of the numerics contract: the forward
@@ -15,6 +16,11 @@ LIBDIR = os.path.join(HERE, 'lib')
 LIB = os.path.join(LIBDIR, 'libuh_hotpath.so')
 SOURCES = ['uh_dlt.hip', 'uh_warp.hip', 'uh_misc.hip', 'uh_patch.hip', 'uh_losses.hip', 'uh_inputs.hip', 'uh_tail.hip', 'uh_epilogue.hip']
 HEADERS = ['uh_device.h', 'uh_host.h', os.path.join('..', '..', 'include', 'uh_hotpath.h')]
+# the operators around the regressor are a library of their own: the hot path's fingerprint (its committed measurements carry
+# it) does not change with them
+MODEL_OPS_LIB = os.path.join(LIBDIR, 'libuh_model_ops.so')
+MODEL_OPS_SOURCES = ['uhm_multi.hip', 'uhm_int8.hip']
+MODEL_OPS_HEADERS = [os.path.join('..', '..', 'include', 'uh_model_ops.h')]
 # `-packed-fp32-ops`: no v_pk_{add,mul,fma}_f32 anywhere -- some of their forms have given wrong results now and then on gfx950.
 # The scalar forms round the same, and every kernel keeps its register count (the warp and patch kernels lose 224 packed
 # instructions, the others had none).  hipcc's host pass warns that it does not know the feature: harmless.
@@ -22,9 +28,9 @@ FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-ffp-contract=off', '-fn
          '-fvisibility=hidden', '-Wall', '-Wno-unused-function', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
-def _fingerprint():
+def _fingerprint(files=None):
     h = hashlib.sha256(' '.join(FLAGS).encode())
-    for f in SOURCES + HEADERS:
+    for f in SOURCES + HEADERS if files is None else files:
         with open(os.path.join(CSRC, f), 'rb') as fh:
             h.update(fh.read())
     return h.hexdigest()
@@ -37,39 +43,50 @@ def find_hipcc():
     raise RuntimeError('hipcc not found: cannot build libuh_hotpath.so')
 
 
-def build_library(force=False, verbose=False):
-    """Compile csrc/*.hip -> lib/libuh_hotpath.so.  Returns the library path."""
+def _build(lib, sources, headers, force, verbose):
     os.makedirs(LIBDIR, exist_ok=True)
-    stamp = LIB + '.sha256'
-    fp = _fingerprint()
-    if not force and os.path.exists(LIB) and os.path.exists(stamp) and open(stamp).read().strip() == fp:
-        return LIB
-    cmd = [find_hipcc()] + FLAGS + [os.path.join(CSRC, s) for s in SOURCES] + ['-o', LIB + '.tmp']
+    stamp = lib + '.sha256'
+    fp = _fingerprint(sources + headers)
+    if not force and os.path.exists(lib) and os.path.exists(stamp) and open(stamp).read().strip() == fp:
+        return lib
+    cmd = [find_hipcc()] + FLAGS + [os.path.join(CSRC, s) for s in sources] + ['-o', lib + '.tmp']
     if verbose:
         print(' '.join(cmd))
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError('hipcc failed:\n' + res.stdout + res.stderr)
-    os.replace(LIB + '.tmp', LIB)
+    os.replace(lib + '.tmp', lib)
     with open(stamp, 'w') as fh:
         fh.write(fp)
-    return LIB
+    return lib
 
 
-def kernel_resources(force=False):
+def build_library(force=False, verbose=False):
+    """Compile csrc/uh_*.hip -> lib/libuh_hotpath.so.  Returns the library path."""
+    return _build(LIB, SOURCES, HEADERS, force, verbose)
+
+
+def build_model_ops(force=False, verbose=False):
+    """Compile csrc/uhm_*.hip -> lib/libuh_model_ops.so.  Returns the library path."""
+    return _build(MODEL_OPS_LIB, MODEL_OPS_SOURCES, MODEL_OPS_HEADERS, force, verbose)
+
+
+def kernel_resources(force=False, sources=None, headers=None):
     """Register / LDS / scratch budget of EVERY kernel of the library, from the code-object metadata hipcc emits
     (`-S --cuda-device-only`: device assembly only, ~10 s for uh_warp.hip, the files in parallel), cached beside the library
     under the same source fingerprint.  -> {demangled kernel name: {'file', 'vgpr', 'agpr', 'sgpr', 'vgpr_spill', 'sgpr_spill',
-    'scratch_bytes', 'lds_bytes', 'dynamic_stack', 'max_threads'}}.  tests/test_kernel_resources.py holds the budgets."""
+    'scratch_bytes', 'lds_bytes', 'dynamic_stack', 'max_threads'}}.  tests/test_kernel_resources.py holds the budgets.
+    sources / headers: those of another library (MODEL_OPS_SOURCES, MODEL_OPS_HEADERS), not cached."""
     import json
     import re
     import tempfile
     from concurrent.futures import ThreadPoolExecutor
     import yaml
     os.makedirs(LIBDIR, exist_ok=True)
-    cache = os.path.join(LIBDIR, 'kernel_resources.json')
-    fp = _fingerprint()
-    if not force and os.path.exists(cache):
+    cache = os.path.join(LIBDIR, 'kernel_resources.json') if sources is None else None
+    sources, headers = (SOURCES, HEADERS) if sources is None else (sources, headers)
+    fp = _fingerprint(sources + headers)
+    if cache and not force and os.path.exists(cache):
         try:
             with open(cache) as fh:
                 c = json.load(fh)
@@ -91,7 +108,7 @@ def kernel_resources(force=False):
             m = re.search(r'\.amdgpu_metadata\n---\n(.*?)\n\.\.\.\n', text, re.S)
             return src, (yaml.safe_load(m.group(1)).get('amdhsa.kernels', []) if m else [])
         with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
-            per_file = list(ex.map(one, SOURCES))
+            per_file = list(ex.map(one, sources))
     names = [k['.name'] for _, ks in per_file for k in ks]
     filt = shutil.which('c++filt')
     dem = subprocess.run([filt] + names, capture_output=True, text=True).stdout.split('\n') if (filt and names) else names
@@ -107,6 +124,8 @@ def kernel_resources(force=False):
                          'scratch_bytes': k.get('.private_segment_fixed_size'), 'lds_bytes': k.get('.group_segment_fixed_size'),
                          'dynamic_stack': bool(k.get('.uses_dynamic_stack', False)),
                          'max_threads': k.get('.max_flat_workgroup_size')}
+    if cache is None:
+        return out
     with open(cache, 'w') as fh:
         json.dump({'fingerprint': fp, 'kernels': out}, fh, indent=0, sort_keys=True)
     return out
@@ -114,3 +133,4 @@ def kernel_resources(force=False):
 
 if __name__ == '__main__':
     print(build_library(force=True, verbose=True))
+    print(build_model_ops(force=True, verbose=True))
