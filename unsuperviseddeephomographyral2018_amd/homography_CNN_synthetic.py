@@ -13,6 +13,7 @@ without it, synthetic.make_batch draws pairs with the same sampling law directly
     torchrun --nproc-per-node 8 -m unsuperviseddeephomographyral2018_amd.homography_CNN_synthetic --batch_size 512
 """
 import argparse
+import contextlib
 import math
 import os
 import time
@@ -22,7 +23,7 @@ import torch
 
 from . import dataloader as uh_data
 from . import dist as uh_dist
-from . import synthetic
+from . import ops, synthetic
 from .homography_model import HomographyModel, VGGRegressor, homography_model_params
 
 # Size of synthetic image and the pertubation range (RH0)      (:14-17)
@@ -94,6 +95,11 @@ def build_parser():
     p.add_argument('--tf_adam_epsilon', type=str2bool, default='True',
                    help='Adam update as tf.train.AdamOptimizer applies it (epsilon = the paper\'s "epsilon hat": homography_CNN_synthetic.tf_adam_eps); '
                         'False = torch.optim.Adam\'s constant eps (rounds 1-5).  --step_graph always uses the latter')
+    p.add_argument('--clip_norm', type=float, default=0.0,
+                   help='> 0: clip the gradients by their global norm before Adam (tf.clip_by_global_norm\'s rule; after averaging over '
+                        'towers), in the same pass over them (ops.adam_clip_update_).  0 = off, as in the reference')
+    p.add_argument('--int8_head', type=str2bool, default='False',
+                   help='test mode: fc1 in 8-bit integers (ops.int8_linear; its weight is quantised per channel, activations per pair)')
     p.add_argument('--tunable_gemm', type=str2bool, default='True',
                    help='PyTorch TunableOp for the fully connected GEMMs (dist.tune_gemms): the first call of each GEMM shape benchmarks '
                         'the rocBLAS / hipBLASLt candidates, as cudnn.benchmark does for the convs (~3 s once per host; fc1 forward '
@@ -187,6 +193,10 @@ class TrainStep(object):
         # the reference's Adam is TF1's ("epsilon hat" form): torch's eps is set per step so that the update is the same (tf_adam_eps).
         # Not in the whole-step hipGraph, where Adam's eps is a captured constant: that mode keeps torch's rule.
         self.tf_adam_epsilon = bool(getattr(args, 'tf_adam_epsilon', True)) and not self.step_graph
+        self.clip_norm = float(getattr(args, 'clip_norm', 0.0))
+        if not self.clip_norm >= 0.0:
+            raise ValueError('--clip_norm must be >= 0 (got %s)' % self.clip_norm)
+        self.grad_norm = None                              # with clip_norm: the last step's global norm (device scalar)
         self.model_params = homography_model_params(
             mode=args.mode, batch_size=int(args.batch_size / world), patch_size=args.patch_size,
             img_h=args.img_h, img_w=args.img_w, loss_type=args.loss_type, use_batch_norm=args.use_batch_norm,
@@ -287,6 +297,30 @@ class TrainStep(object):
         torch.distributed.barrier()
         return time.perf_counter() - t0
 
+    def _update(self):
+        """Adam, with clip_norm after clipping by the global norm.  The eager step clips on the way (the gradients are not written
+        back); in the whole-step graph, where Adam's scalars live on the device, they are clipped in place."""
+        if self.clip_norm == 0.0:
+            self.opt.step()
+            return
+        group = self.opt.param_groups[0]
+        params = [p for p in group['params'] if p.grad is not None]
+        if self.step_graph:
+            self.grad_norm = ops.clip_by_global_norm_([p.grad for p in params], self.clip_norm)
+            self.opt.step()
+            return
+        states = [self.opt.state[p] for p in params]
+        for p, st in zip(params, states):
+            if not st:                                      # as torch.optim.Adam(fused=True) lays its state out: one checkpoint format
+                st['step'] = torch.zeros((), dtype=torch.float32, device=p.device)
+                st['exp_avg'] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                st['exp_avg_sq'] = torch.zeros_like(p, memory_format=torch.preserve_format)
+        beta1, beta2 = group['betas']
+        self.grad_norm = ops.adam_clip_update_(params, [p.grad for p in params], [st['exp_avg'] for st in states],
+                                               [st['exp_avg_sq'] for st in states], lr=group['lr'], beta1=beta1, beta2=beta2,
+                                               eps=group['eps'], step=self.adam_t + 1, clip_norm=self.clip_norm)
+        torch._foreach_add_([st['step'] for st in states], 1.0)
+
     def _forward_backward_update(self, batch):
         self._zero_or_reset()
         model = HomographyModel(self.model_params, *synthetic.model_args(batch), reuse_variables=True,
@@ -295,7 +329,7 @@ class TrainStep(object):
         model.loss.backward()
         if self.averager is not None:
             self.averager.finish()
-        self.opt.step()
+        self._update()
         return model
 
     def __call__(self, batch):
@@ -336,7 +370,7 @@ class TrainStep(object):
         model.loss.backward()
         if self.averager is not None:
             self.averager.finish()
-        self.opt.step()
+        self._update()
         self.global_step += 1
         self.adam_t += 1
         return model
@@ -451,6 +485,7 @@ def train(args):
                     print('Train: step %d  ' % step + ', '.join('%s %.6f' % (kk, v) for kk, v in zip(names, avg))
                           + ', lr %.6f, %.1f pairs/s' % (step_fn.learning_rate(), n * args.batch_size / max(dt, 1e-9))
                           + '  | last %d steps: h_loss %.4f %s %.6f' % (mon['win_n'], win[0], args.loss_type, win[names.index(args.loss_type)])
+                          + ('  | gradient norm %.4g' % float(step_fn.grad_norm) if step_fn.grad_norm is not None else '')
                           + ('  | %d tower-steps with a non-finite loss value so far' % mon['nonfinite'] if mon['nonfinite'] else '')
                           + ('  | %d pairs had a non-finite gradient zeroed so far (--zero_nonfinite_grad; the reference would have '
                              'propagated NaN)' % zeroed_pairs if zeroed_pairs else ''),
@@ -570,7 +605,8 @@ class TestHomography(object):
         num_steps = 3 * steps_per_epoch                                   # (:400-401)
         per_pair, per_step, total_fail, total_bounded = [], [], 0.0, 0.0
         was_training = self.net.training
-        with torch.no_grad():
+        head = self.net.int8_head() if getattr(a, 'int8_head', False) else contextlib.nullcontext()
+        with torch.no_grad(), head:
             for step in range(num_steps):
                 batch = next(disk) if disk is not None else synthetic.make_batch(
                     a.batch_size, a.img_h, a.img_w, a.patch_size, a.rho, seed=10_000_000 + a.seed + step,

@@ -11,6 +11,7 @@ What runs where
     of the one being trained on: the HIP C-ABI library via ops.py -- no torch math (the supervised h_loss that
     carries a gradient, :288, is one torch expression on [B,8]).
 """
+import contextlib
 from collections import namedtuple
 
 import numpy as np
@@ -63,6 +64,7 @@ class VGGRegressor(nn.Module):
         self.dropout_p = dropout_p
         # conv GEMMs on stock MIOpen; bias + ReLU (+ their backward and the bias gradient) as one HIP pass each
         self.fused_epilogue = fused_epilogue
+        self._int8_fc1 = None                        # (weight, scales, bias) within int8_head()
         chans = [(2, 64), (64, 64), (64, 64), (64, 64), (64, 128), (128, 128), (128, 128), (128, 128)]
         self.convs = nn.ModuleList([nn.Conv2d(i, o, 3, stride=1, padding=1) for i, o in chans])
         self.use_batch_norm = use_batch_norm
@@ -94,6 +96,23 @@ class VGGRegressor(nn.Module):
             x = self.bns[i](x)
         return x
 
+    @contextlib.contextmanager
+    def int8_head(self):
+        """Within it, evaluation computes fc1 in 8-bit integers (ops.int8_linear).  The weight is quantised on entry, one scale per
+        channel, and read as 33 MB instead of 134; training mode stays in float32.  No gradient: call under torch.no_grad()."""
+        w, scale = ops.quantize_rows(self.fc1.weight.detach())
+        self._int8_fc1, before = (w, scale, self.fc1.bias.detach()), self._int8_fc1
+        try:
+            yield self
+        finally:
+            self._int8_fc1 = before
+
+    def _fc1_relu(self, x):
+        if self._int8_fc1 is None or self.training:
+            return F.relu(self.fc1(x))
+        w, scale, bias = self._int8_fc1
+        return ops.int8_linear(x, w, scale, bias=bias, relu=True)
+
     def forward(self, model_input_nhwc):
         # [B,P,P,2] NHWC -> NCHW-logical view with channels_last strides (no copy)
         x = model_input_nhwc.permute(0, 3, 1, 2)
@@ -103,7 +122,7 @@ class VGGRegressor(nn.Module):
         x = self._conv(self._conv(x, 6), 7)
         x = F.dropout(x, self.dropout_p, self.training)
         x = x.permute(0, 2, 3, 1).reshape(x.shape[0], -1)          # slim.flatten of NHWC
-        x = F.dropout(F.relu(self.fc1(x)), self.dropout_p, self.training)
+        x = F.dropout(self._fc1_relu(x), self.dropout_p, self.training)
         return self.fc2(x)
 
 
