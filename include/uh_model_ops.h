@@ -105,6 +105,13 @@ UHM_API int uhm_int8_matmul(const int8_t* a, long long a_ld, const float* a_scal
                             const float* b_scale, const float* bias, void* out, int out_dtype, long long M, long long N, long long K,
                             unsigned flags, void* workspace, size_t workspace_bytes, uhm_stream_t stream);
 
+/* The layer on float tokens: rows of x [M, K] (row stride x_ld in elements) quantised as uhm_quantize_rows does, the product as
+ * uhm_int8_matmul computes it (the same bits), out [M, N] of x's type.  One row: a single launch.  Workspace: 16-byte aligned.   */
+UHM_API size_t uhm_int8_linear_workspace_bytes(long long M, long long N, long long K);
+UHM_API int uhm_int8_linear(const void* x, int dtype, long long x_ld, const int8_t* b, long long b_ld, const float* b_scale,
+                            const float* bias, void* out, long long M, long long N, long long K, unsigned flags, void* workspace,
+                            size_t workspace_bytes, uhm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -86,6 +86,8 @@ MODEL_OPS_SIGNATURES = {
     'uhm_quantize_rows': (_i, [_p, _i, _q, _p, _q, _p, _q, _q, _p]),
     'uhm_int8_matmul_workspace_bytes': (_z, [_q, _q, _q]),
     'uhm_int8_matmul': (_i, [_p, _q, _p, _p, _q, _p, _p, _p, _i, _q, _q, _q, _u, _p, _z, _p]),
+    'uhm_int8_linear_workspace_bytes': (_z, [_q, _q, _q]),
+    'uhm_int8_linear': (_i, [_p, _i, _q, _p, _q, _p, _p, _p, _q, _q, _q, _u, _p, _z, _p]),
 }
 
 _lib = None

@@ -3,7 +3,7 @@
 //   quantise:  top = max |x_r|, scale_r = top / 127, q = rne(x * (127 / top))
 //   product :  out[m, n] = act(sum_k a[m, k] b[n, k] * sa[m] * sb[n] + bias[n])        exact 32-bit integer sums
 //
-// One tiled kernel for every size, on v_mfma_i32_32x32x32_i8.  A block computes BM x BN outputs over a range of K: tiles of
+// Up to FEW tokens: int8_few_kernel, which streams the weight once.  More: one tiled kernel on v_mfma_i32_32x32x32_i8.  A block computes BM x BN outputs over a range of K: tiles of
 // BK = 128 bytes of BM rows of a and BN rows of b go global -> registers -> LDS (two buffers; the next tile's loads are in flight
 // while the present one is multiplied, one barrier per tile).  A tile row is 128 bytes = 8 chunks of 16; chunk c of row r sits at
 // position c ^ (r & 7), so that the 8 rows that 8 lanes read at once (one chunk each) cover all 64 banks' 128 bytes, and so does
@@ -13,6 +13,7 @@
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
+#include <type_traits>
 #include "../../include/uh_model_ops.h"
 
 namespace uhm {
@@ -162,25 +163,26 @@ __global__ __launch_bounds__(WM * WN * 64) void int8_matmul_kernel(const int8_t*
     }
 }
 
-// joins the splits: out[m, n] from sum_s sums[s][m][n]
+// joins the splits: out[m, n] from sum_s sums[s][m][n].  The loads of 16 splits are in flight together (one after the other each
+// waits for a trip to the L2 or beyond: 64 splits took 16 us that way).
 __global__ __launch_bounds__(256) void int8_join_kernel(const int* __restrict__ sums, int splits, int M, int N, const Epilogue e) {
     const size_t total = (size_t)M * N;
     for (size_t at = (size_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (size_t)gridDim.x * 256) {
         const int m = (int)(at / N), n = (int)(at - (size_t)m * N);
+        const float sam = e.a_scale[m], sbn = e.b_scale[n], bias = e.bias ? e.bias[n] : 0.f;
         int acc = 0;
-        for (int s = 0; s < splits; ++s) acc += sums[s * total + at];
-        put(e.out, e.dtype, at, finish(acc, e.a_scale[m], e.b_scale[n], e.bias ? e.bias[n] : 0.f, e.relu));
+        for (int s = 0; s < splits; s += 16) {
+            int v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = s + j < splits ? sums[(size_t)(s + j) * total + at] : 0;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc += v[j];
+        }
+        put(e.out, e.dtype, at, finish(acc, sam, sbn, bias, e.relu));
     }
 }
 
 // ---- rows to 8 bits -----------------------------------------------------------------------------------------------------------
-template <int T>
-__device__ __forceinline__ float value(const void* x, size_t i) {
-    if constexpr (T == UHM_F32) return ((const float*)x)[i];
-    else if constexpr (T == UHM_BF16) return __uint_as_float((unsigned)((const unsigned short*)x)[i] << 16);
-    else return __half2float(__ushort_as_half(((const unsigned short*)x)[i]));
-}
-
 struct RowScale { float scale, inverse; };
 // `bits`: the largest |x| as an integer (the order of non-negative floats; infinities and NaN are above all numbers)
 __device__ __forceinline__ RowScale row_scale(unsigned bits) {
@@ -190,37 +192,190 @@ __device__ __forceinline__ RowScale row_scale(unsigned bits) {
     return {top / 127.0f, 127.0f / top};
 }
 // round to nearest even of the exact product: adding 1.5 * 2^23 leaves the integer in the low bits, with one rounding (fma)
-__device__ __forceinline__ int quantise(float x, RowScale s) {
+__device__ __forceinline__ unsigned quantise(float x, RowScale s) {
     if (s.inverse == 0.f) return 0;
-    return (int)(__float_as_uint(fmaf(x, s.inverse, 0x1.8p23f)) & 0xffu);
+    return __float_as_uint(fmaf(x, s.inverse, 0x1.8p23f)) & 0xffu;
+}
+struct F4 { float v[4]; };
+__device__ __forceinline__ unsigned quantise4(const F4& x, RowScale s) {
+    return quantise(x.v[0], s) | quantise(x.v[1], s) << 8 | quantise(x.v[2], s) << 16 | quantise(x.v[3], s) << 24;
+}
+__device__ __forceinline__ unsigned top_of(const F4& x) {
+    unsigned t = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t = max(t, __float_as_uint(x.v[j]) & 0x7fffffffu);
+    return t;
 }
 
+template <int T> struct Raw { using type = unsigned short; };
+template <> struct Raw<UHM_F32> { using type = float; };
 template <int T>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(const void* __restrict__ x, long long x_ld, int8_t* __restrict__ q,
-                                                            long long q_ld, float* __restrict__ scale, int K) {
-    __shared__ unsigned sm[4];
-    const size_t row = blockIdx.x;
-    const char* px = (const char*)x + row * x_ld * (T == UHM_F32 ? 4 : 2);
-    unsigned top = 0;
-    for (int k = threadIdx.x; k < K; k += 256) top = max(top, __float_as_uint(value<T>(px, k)) & 0x7fffffffu);
+__device__ __forceinline__ float value(typename Raw<T>::type r) {
+    if constexpr (T == UHM_F32) return r;
+    else if constexpr (T == UHM_BF16) return __uint_as_float((unsigned)r << 16);
+    else return __half2float(__ushort_as_half(r));
+}
+// elements k .. k + 3 of a row, zeros behind K (k % 4 == 0).  `aligned`: the row starts on four elements
+template <int T>
+__device__ __forceinline__ F4 load4(const void* row, int k, int K, bool aligned) {
+    using raw = typename Raw<T>::type;
+    struct alignas(4 * sizeof(raw)) R4 { raw v[4]; };
+    const raw* p = (const raw*)row + k;
+    F4 x = {{0.f, 0.f, 0.f, 0.f}};
+    if (aligned && k + 4 <= K) {
+        const R4 r = *reinterpret_cast<const R4*>(p);
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, d, 64));
-    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = top;
-    __syncthreads();
-    const RowScale s = row_scale(max(max(sm[0], sm[1]), max(sm[2], sm[3])));
-    if (threadIdx.x == 0) scale[row] = s.scale;
-    int8_t* pq = q + row * q_ld;
-    for (int k = threadIdx.x * 4; k < (K + 15) / 16 * 16; k += 1024) {
-        unsigned w = 0;
+        for (int j = 0; j < 4; ++j) x.v[j] = value<T>(r.v[j]);
+    } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (k + j < K) w |= (unsigned)quantise(value<T>(px, k + j), s) << (8 * j);
-        *reinterpret_cast<unsigned*>(pq + k) = w;
+            if (k + j < K) x.v[j] = value<T>(p[j]);
+    }
+    return x;
+}
+
+// the largest of `top` over a block of T threads, in every thread
+template <int T>
+__device__ __forceinline__ unsigned block_max(unsigned top) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, d, 64));
+    if constexpr (T > 64) {
+        __shared__ unsigned sm[T / 64];
+        if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < T / 64; ++w) top = max(top, sm[w]);
+    }
+    return top;
+}
+
+// One block per row.  Bound by the reads of x; a row of up to 32 T values stays in registers between the maximum and the rounding,
+// a longer one is read a second time (out of the L2).  All of a thread's loads are in flight together.
+template <int X, int T>
+__global__ __launch_bounds__(T) void quantize_rows_kernel(const void* __restrict__ x, long long x_ld, int8_t* __restrict__ q,
+                                                          long long q_ld, float* __restrict__ scale, int K, int aligned) {
+    constexpr int HELD = 8;
+    const size_t row = blockIdx.x;
+    const char* px = (const char*)x + row * x_ld * sizeof(typename Raw<X>::type);
+    const int padded = (K + 15) & ~15;
+    F4 held[HELD];
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) held[i] = load4<X>(px, min(threadIdx.x + i * T, (unsigned)(padded - 1) / 4) * 4, K, aligned);
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) top = max(top, top_of(held[i]));
+    for (int k = (HELD * T + threadIdx.x) * 4; k < K; k += T * 4) top = max(top, top_of(load4<X>(px, k, K, aligned)));
+    const RowScale s = row_scale(block_max<T>(top));
+    if (threadIdx.x == 0) scale[row] = s.scale;
+    int8_t* pq = q + row * q_ld;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        const int k = (threadIdx.x + i * T) * 4;
+        if (k < padded) *reinterpret_cast<unsigned*>(pq + k) = quantise4(held[i], s);
+    }
+    for (int k = (HELD * T + threadIdx.x) * 4; k < padded; k += T * 4)
+        *reinterpret_cast<unsigned*>(pq + k) = quantise4(load4<X>(px, k, K, aligned), s);
+}
+
+// ---- few tokens -----------------------------------------------------------------------------------------------------------------
+// Up to MB tokens per block: bound by the one read of the weight.  A block of T threads owns R channels and all of K (no split, no
+// join, one launch): thread t holds bytes 16 t .. 16 t + 15 of every T * 16, AHEAD steps of every channel's row are in flight, products on
+// the 4-way dot instruction (for so few tokens they take less time than the loads).  X < 0: tokens in 8 bits.  X >= 0: ONE token
+// of that float type, quantised here: every block finds the row's maximum again (the row comes out of the L2) while its weight
+// loads are on their way, and rounds its chunks as it needs them.
+template <int T, int R, int MB, int X>
+__global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x, long long x_ld, int aligned, const int8_t* __restrict__ b,
+                                                     long long b_ld, int M, int N, int K, const Epilogue e) {
+    static_assert(X < 0 || MB == 1, "one token");
+    constexpr int STEP = T * 16, AHEAD = R * MB >= 16 ? 2 : 4;
+    const int tid = threadIdx.x;
+    const long long n0 = (long long)blockIdx.x * R;
+    const int m0 = blockIdx.y * MB;
+    const int8_t* pb[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) pb[r] = b + min(n0 + r, (long long)N - 1) * b_ld;
+    v4i w[AHEAD][R];
+    auto fetch = [&](int p, int k) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) w[p][r] = load16(pb[r], k, K, false);
+    };
+#pragma unroll
+    for (int p = 0; p < AHEAD; ++p) fetch(p, p * STEP + tid * 16);
+
+    RowScale s = {0.f, 0.f};
+    const int8_t* px[MB];
+    if constexpr (X >= 0) {
+        unsigned top = 0;
+        for (int k = tid * 4; k < K; k += 32 * T) {
+            F4 h[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[i] = load4<X>(x, min(k + i * T * 4, (K - 1) & ~3), K, aligned);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = max(top, top_of(h[i]));
+        }
+        s = row_scale(block_max<T>(top));
+    } else {
+#pragma unroll
+        for (int m = 0; m < MB; ++m) px[m] = (const int8_t*)x + min(m0 + m, M - 1) * x_ld;
+    }
+
+    int acc[R][MB];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int m = 0; m < MB; ++m) acc[r][m] = 0;
+    for (int base = 0; base < K; base += AHEAD * STEP) {
+#pragma unroll
+        for (int p = 0; p < AHEAD; ++p) {
+            const int k = base + p * STEP + tid * 16;
+            v4i xv[MB];
+            if constexpr (X >= 0) {
+                xv[0] = v4i{0, 0, 0, 0};
+                if (k < K) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) xv[0][j] = (int)quantise4(load4<X>(x, k + 4 * j, K, aligned), s);
+                }
+            } else {
+#pragma unroll
+                for (int m = 0; m < MB; ++m) xv[m] = load16(px[m], k, K, true);
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int m = 0; m < MB; ++m)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[r][m] = __builtin_amdgcn_sdot4(w[p][r][j], xv[m][j], acc[r][m], false);
+            if (k + AHEAD * STEP < K) fetch(p, k + AHEAD * STEP);      // (what it leaves stale meets zeros)
+        }
+    }
+
+    constexpr int WAVES = T / 64;
+    __shared__ int sm[WAVES][R * MB];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            int v = acc[r][m];
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+            if ((tid & 63) == 0) sm[tid >> 6][r * MB + m] = v;
+        }
+    __syncthreads();
+    if (tid < R * MB) {
+        const int r = tid / MB, m = tid % MB;
+        const long long n = n0 + r;
+        if (n < N && m0 + m < M) {
+            int v = 0;
+#pragma unroll
+            for (int wv = 0; wv < WAVES; ++wv) v += sm[wv][tid];
+            put(e.out, e.dtype, (size_t)(m0 + m) * N + n, finish(v, X >= 0 ? s.scale : e.a_scale[m0 + m], e.b_scale[n], e.bias ? e.bias[n] : 0.f, e.relu));
+        }
     }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 constexpr long long MAX_K = 131071, MAX_DIM = 0x7fffffffLL - 512;
+constexpr long long FEW = 4;               // tokens up to which the weight is read by int8_few_kernel
 
 struct Plan { int bm, bn, splits, tiles_per_split; };
 
@@ -249,54 +404,65 @@ int check_product(long long M, long long N, long long K) {
     return 0;
 }
 
-}  // namespace uhm
-
-using namespace uhm;
-
-extern "C" int uhm_quantize_rows(const void* x, int dtype, long long x_ld, int8_t* q, long long q_ld, float* scale, long long rows,
-                                 long long K, uhm_stream_t stream) {
-    if (rows < 0 || K < 1 || x_ld < K || q_ld < K) return UHM_E_SHAPE;
-    if (rows > MAX_DIM || K > MAX_DIM) return UHM_E_TOO_LARGE;
-    if (dtype < UHM_F32 || dtype > UHM_F16) return UHM_E_DTYPE;
-    if (rows == 0) return 0;
-    if (!x || !q || !scale) return UHM_E_NULL;
-    if (((uintptr_t)q & 15) || (q_ld & 15) || ((uintptr_t)x & (dtype == UHM_F32 ? 3 : 1)) || ((uintptr_t)scale & 3)) return UHM_E_ALIGN;
-    hipStream_t s = (hipStream_t)stream;
-    const dim3 grid((unsigned)rows), block(256);
-    if (dtype == UHM_F32) hipLaunchKernelGGL(quantize_rows_kernel<UHM_F32>, grid, block, 0, s, x, x_ld, q, q_ld, scale, (int)K);
-    else if (dtype == UHM_BF16) hipLaunchKernelGGL(quantize_rows_kernel<UHM_BF16>, grid, block, 0, s, x, x_ld, q, q_ld, scale, (int)K);
-    else hipLaunchKernelGGL(quantize_rows_kernel<UHM_F16>, grid, block, 0, s, x, x_ld, q, q_ld, scale, (int)K);
-    return (int)hipGetLastError();
-}
-
-extern "C" size_t uhm_int8_matmul_workspace_bytes(long long M, long long N, long long K) {
-    if (check_product(M, N, K) || M == 0 || N == 0) return 0;
-    const Plan p = plan_of(M, N, K);
-    return p.splits > 1 ? (size_t)p.splits * M * N * sizeof(int) : 0;
-}
-
-extern "C" int uhm_int8_matmul(const int8_t* a, long long a_ld, const float* a_scale, const int8_t* b, long long b_ld,
-                               const float* b_scale, const float* bias, void* out, int out_dtype, long long M, long long N, long long K,
-                               unsigned flags, void* workspace, size_t workspace_bytes, uhm_stream_t stream) {
+// what the entry points for products check alike (x: the tokens, in 8 bits or as floats)
+int check_operands(const void* x, long long x_ld, const int8_t* b, long long b_ld, const float* b_scale, const float* bias, const void* out,
+                   int out_dtype, long long M, long long N, long long K, unsigned flags) {
     if (int err = check_product(M, N, K)) return err;
-    if (a_ld < K || b_ld < K) return UHM_E_SHAPE;
+    if (x_ld < K || b_ld < K) return UHM_E_SHAPE;
     if (out_dtype < UHM_F32 || out_dtype > UHM_F16) return UHM_E_DTYPE;
     if (flags & ~UHM_RELU) return UHM_E_VALUE;
     if (M == 0 || N == 0) return 0;
-    if (!a || !a_scale || !b || !b_scale || !out) return UHM_E_NULL;
-    if ((((uintptr_t)a | (uintptr_t)b | (uintptr_t)a_ld | (uintptr_t)b_ld) & 15) ||
-        (((uintptr_t)a_scale | (uintptr_t)b_scale | (uintptr_t)bias) & 3) || ((uintptr_t)out & (out_dtype == UHM_F32 ? 3 : 1)))
+    if (!x || !b || !b_scale || !out) return UHM_E_NULL;
+    if ((((uintptr_t)b | (uintptr_t)b_ld) & 15) || (((uintptr_t)b_scale | (uintptr_t)bias) & 3) || ((uintptr_t)out & (out_dtype == UHM_F32 ? 3 : 1)))
         return UHM_E_ALIGN;
+    return 0;
+}
+
+// the row starts on four elements
+inline int rows_aligned(const void* x, int dtype, long long x_ld, long long rows) {
+    const uintptr_t size = dtype == UHM_F32 ? 4 : 2;
+    return (((uintptr_t)x | (rows > 1 ? (uintptr_t)x_ld * size : 0)) & (4 * size - 1)) == 0;
+}
+
+template <int X>
+int quantize_rows(const void* x, long long x_ld, int8_t* q, long long q_ld, float* scale, long long rows, long long K, hipStream_t s) {
+    const int al = rows_aligned(x, X, x_ld, rows);
+    // as few threads as hold the row in registers
+    auto launch = [&](auto kernel, int threads) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(threads), 0, s, x, x_ld, q, q_ld, scale, (int)K, al);
+    };
+    if (K <= 2048) launch(quantize_rows_kernel<X, 64>, 64);
+    else if (K <= 8192) launch(quantize_rows_kernel<X, 256>, 256);
+    else launch(quantize_rows_kernel<X, 1024>, 1024);
+    return (int)hipGetLastError();
+}
+
+template <int MB, int X>
+int launch_few(const void* x, long long x_ld, int al, const int8_t* b, long long b_ld, int M, int N, int K, const Epilogue& e, hipStream_t s) {
+    auto launch = [&](auto kernel, int threads, int R) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(((long long)N + R - 1) / R), (unsigned)((M + MB - 1) / MB)), dim3(threads), 0, s, x, x_ld, al, b, b_ld, M, N, K, e);
+    };
+    // threads by K (two to four steps of 16 bytes each), channels per block by N: at least a block for every CU before a block takes more
+    auto rows = [&](auto t) {
+        constexpr int T = decltype(t)::value;
+        if (N >= 1024) launch(int8_few_kernel<T, 4, MB, X>, T, 4);
+        else if (N >= 512) launch(int8_few_kernel<T, 2, MB, X>, T, 2);
+        else launch(int8_few_kernel<T, 1, MB, X>, T, 1);
+    };
+    if (K <= 2048) rows(std::integral_constant<int, 64>{});
+    else if (K <= 16384) rows(std::integral_constant<int, 256>{});
+    else rows(std::integral_constant<int, 512>{});
+    return (int)hipGetLastError();
+}
+
+int product(const int8_t* a, long long a_ld, const int8_t* b, long long b_ld, long long M, long long N, long long K, const Epilogue& e, int* sums,
+            hipStream_t s) {
+    if (M <= 1) return launch_few<1, -1>(a, a_ld, 1, b, b_ld, (int)M, (int)N, (int)K, e, s);
+    if (M <= 2) return launch_few<2, -1>(a, a_ld, 1, b, b_ld, (int)M, (int)N, (int)K, e, s);
+    if (M <= FEW) return launch_few<4, -1>(a, a_ld, 1, b, b_ld, (int)M, (int)N, (int)K, e, s);
     const Plan p = plan_of(M, N, K);
-    int* sums = nullptr;
-    if (p.splits > 1) {
-        if (!workspace || workspace_bytes < uhm_int8_matmul_workspace_bytes(M, N, K)) return UHM_E_WORKSPACE;
-        if ((uintptr_t)workspace & 15) return UHM_E_ALIGN;
-        sums = (int*)workspace;
-    }
-    const Epilogue e = {a_scale, b_scale, bias, out, out_dtype, (flags & UHM_RELU) ? 1 : 0};
-    hipStream_t s = (hipStream_t)stream;
     const dim3 grid((unsigned)((N + p.bn - 1) / p.bn), (unsigned)((M + p.bm - 1) / p.bm), (unsigned)p.splits);
+    if (p.splits == 1) sums = nullptr;
     auto launch = [&](auto kernel, int threads) {
         hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, a, a_ld, b, b_ld, (int)M, (int)N, (int)K, p.tiles_per_split, sums, e);
     };
@@ -311,4 +477,90 @@ extern "C" int uhm_int8_matmul(const int8_t* a, long long a_ld, const float* a_s
         return (int)hipGetLastError();
     }
     return 0;
+}
+
+size_t sums_bytes(long long M, long long N, long long K) {
+    if (M <= FEW) return 0;
+    const Plan p = plan_of(M, N, K);
+    return p.splits > 1 ? (size_t)p.splits * M * N * sizeof(int) : 0;
+}
+
+// workspace of a layer on float tokens: rows in 8 bits, their scales, the partial sums
+struct LinearSpace { long long q_ld; size_t scale, sums, total; };
+LinearSpace linear_space(long long M, long long N, long long K) {
+    LinearSpace w;
+    w.q_ld = (K + 127) / 128 * 128;                              // rows start on 128 bytes
+    w.scale = (size_t)M * w.q_ld;
+    w.sums = (w.scale + M * sizeof(float) + 127) / 128 * 128;
+    w.total = w.sums + sums_bytes(M, N, K);
+    return w;
+}
+
+int check_space(const void* workspace, size_t bytes, size_t need) {
+    if (!need) return 0;
+    if (!workspace || bytes < need) return UHM_E_WORKSPACE;
+    return ((uintptr_t)workspace & 15) ? UHM_E_ALIGN : 0;
+}
+
+}  // namespace uhm
+
+using namespace uhm;
+
+extern "C" int uhm_quantize_rows(const void* x, int dtype, long long x_ld, int8_t* q, long long q_ld, float* scale, long long rows,
+                                 long long K, uhm_stream_t stream) {
+    if (rows < 0 || K < 1 || x_ld < K || q_ld < K) return UHM_E_SHAPE;
+    if (rows > MAX_DIM || K > MAX_DIM - 8192) return UHM_E_TOO_LARGE;      // (a thread's index goes one step past K)
+    if (dtype < UHM_F32 || dtype > UHM_F16) return UHM_E_DTYPE;
+    if (rows == 0) return 0;
+    if (!x || !q || !scale) return UHM_E_NULL;
+    if (((uintptr_t)q & 15) || (q_ld & 15) || ((uintptr_t)x & (dtype == UHM_F32 ? 3 : 1)) || ((uintptr_t)scale & 3)) return UHM_E_ALIGN;
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == UHM_F32) return quantize_rows<UHM_F32>(x, x_ld, q, q_ld, scale, rows, K, s);
+    if (dtype == UHM_BF16) return quantize_rows<UHM_BF16>(x, x_ld, q, q_ld, scale, rows, K, s);
+    return quantize_rows<UHM_F16>(x, x_ld, q, q_ld, scale, rows, K, s);
+}
+
+extern "C" size_t uhm_int8_matmul_workspace_bytes(long long M, long long N, long long K) {
+    if (check_product(M, N, K) || M == 0 || N == 0) return 0;
+    return sums_bytes(M, N, K);
+}
+
+extern "C" int uhm_int8_matmul(const int8_t* a, long long a_ld, const float* a_scale, const int8_t* b, long long b_ld,
+                               const float* b_scale, const float* bias, void* out, int out_dtype, long long M, long long N, long long K,
+                               unsigned flags, void* workspace, size_t workspace_bytes, uhm_stream_t stream) {
+    if (int err = check_operands(a, a_ld, b, b_ld, b_scale, bias, out, out_dtype, M, N, K, flags)) return err;
+    if (M == 0 || N == 0) return 0;
+    if (!a_scale) return UHM_E_NULL;
+    if ((((uintptr_t)a | (uintptr_t)a_ld) & 15) || ((uintptr_t)a_scale & 3)) return UHM_E_ALIGN;
+    if (int err = check_space(workspace, workspace_bytes, sums_bytes(M, N, K))) return err;
+    const Epilogue e = {a_scale, b_scale, bias, out, out_dtype, (flags & UHM_RELU) ? 1 : 0};
+    return product(a, a_ld, b, b_ld, M, N, K, e, (int*)workspace, (hipStream_t)stream);
+}
+
+extern "C" size_t uhm_int8_linear_workspace_bytes(long long M, long long N, long long K) {
+    if (check_product(M, N, K) || M <= 1 || N == 0) return 0;
+    return linear_space(M, N, K).total;
+}
+
+extern "C" int uhm_int8_linear(const void* x, int dtype, long long x_ld, const int8_t* b, long long b_ld, const float* b_scale,
+                               const float* bias, void* out, long long M, long long N, long long K, unsigned flags, void* workspace,
+                               size_t workspace_bytes, uhm_stream_t stream) {
+    if (int err = check_operands(x, x_ld, b, b_ld, b_scale, bias, out, dtype, M, N, K, flags)) return err;
+    if (M == 0 || N == 0) return 0;
+    if ((uintptr_t)x & (dtype == UHM_F32 ? 3 : 1)) return UHM_E_ALIGN;
+    hipStream_t s = (hipStream_t)stream;
+    Epilogue e = {nullptr, b_scale, bias, out, dtype, (flags & UHM_RELU) ? 1 : 0};
+    if (M == 1) {
+        const int al = rows_aligned(x, dtype, x_ld, 1);
+        if (dtype == UHM_F32) return launch_few<1, UHM_F32>(x, x_ld, al, b, b_ld, 1, (int)N, (int)K, e, s);
+        if (dtype == UHM_BF16) return launch_few<1, UHM_BF16>(x, x_ld, al, b, b_ld, 1, (int)N, (int)K, e, s);
+        return launch_few<1, UHM_F16>(x, x_ld, al, b, b_ld, 1, (int)N, (int)K, e, s);
+    }
+    const LinearSpace w = linear_space(M, N, K);
+    if (int err = check_space(workspace, workspace_bytes, w.total)) return err;
+    int8_t* q = (int8_t*)workspace;
+    float* scale = (float*)((char*)workspace + w.scale);
+    if (int err = uhm_quantize_rows(x, dtype, x_ld, q, w.q_ld, scale, M, K, stream)) return err;
+    e.a_scale = scale;
+    return product(q, w.q_ld, b, b_ld, M, N, K, e, (int*)((char*)workspace + w.sums), s);
 }

@@ -989,21 +989,17 @@ def _row_scales(scale, rows, device, name):
     return scale
 
 
-def _int8_product(lib, a, a_ld, a_scale, M, weight, weight_scale, bias, relu, dtype, K, stream):
-    device = a_scale.device
-    w2, wlead, N, wK, w_ld = _int8_rows(weight, 'weight')
-    if len(wlead) != 1 or wK != K or w2.device != device:
+def _weight_of(weight, weight_scale, bias, K, device):
+    w2, lead, N, wK, w_ld = _int8_rows(weight, 'weight')
+    if len(lead) != 1 or wK != K or w2.device != device:
         raise _lib.UHError('weight must be int8 [N, %d] on %s (got %s on %s)' % (K, device, tuple(weight.shape), weight.device))
-    w_scale = _row_scales(weight_scale, N, device, 'weight_scale')
     if bias is not None:
         bias = _row_scales(bias, N, device, 'bias')
-    out = torch.empty((M, N), dtype=dtype, device=device)
-    nbytes = lib.uhm_int8_matmul_workspace_bytes(M, N, K)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
-    _lib.check_model(lib.uhm_int8_matmul(a.data_ptr(), a_ld, a_scale.data_ptr(), w2.data_ptr(), w_ld, w_scale.data_ptr(), _ptr(bias),
-                                         out.data_ptr(), _UHM_DTYPES[dtype], M, N, K, _lib.UHM_RELU if relu else 0, _ptr(ws), nbytes,
-                                         stream), 'uhm_int8_matmul')
-    return out
+    return w2, w_ld, N, _row_scales(weight_scale, N, device, 'weight_scale'), bias
+
+
+def _workspace(nbytes, device):
+    return torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
 
 
 def int8_matmul(x, x_scale, weight, weight_scale, bias=None, relu=False, out_dtype=torch.float32):
@@ -1016,9 +1012,15 @@ def int8_matmul(x, x_scale, weight, weight_scale, bias=None, relu=False, out_dty
     _no_grad_wanted([t for t in (x_scale, weight_scale, bias) if isinstance(t, torch.Tensor)], 'int8_matmul')
     x2, lead, M, K, x_ld = _int8_rows(x, 'x')
     x_scale = _row_scales(x_scale, M, x2.device, 'x_scale')
+    w, w_ld, N, w_scale, bias = _weight_of(weight, weight_scale, bias, K, x2.device)
     with _on_device(x2.device) as stream:
-        out = _int8_product(lib, x2, x_ld, x_scale, M, weight, weight_scale, bias, relu, out_dtype, K, stream)
-    return out.view(*lead, out.shape[1])
+        out = torch.empty(lead + (N,), dtype=out_dtype, device=x2.device)
+        nbytes = lib.uhm_int8_matmul_workspace_bytes(M, N, K)
+        ws = _workspace(nbytes, x2.device)
+        _lib.check_model(lib.uhm_int8_matmul(x2.data_ptr(), x_ld, x_scale.data_ptr(), w.data_ptr(), w_ld, w_scale.data_ptr(), _ptr(bias),
+                                             out.data_ptr(), _UHM_DTYPES[out_dtype], M, N, K, _lib.UHM_RELU if relu else 0, _ptr(ws),
+                                             nbytes, stream), 'uhm_int8_matmul')
+    return out
 
 
 def int8_linear(x, weight, weight_scale, bias=None, relu=False):
@@ -1028,7 +1030,13 @@ def int8_linear(x, weight, weight_scale, bias=None, relu=False):
     lib = _lib.load_model_ops()
     x2, lead, K, dtype = _float_rows(x, 'x')
     _no_grad_wanted([t for t in (x, weight_scale, bias) if isinstance(t, torch.Tensor)], 'int8_linear')
+    M = x2.shape[0]
+    w, w_ld, N, w_scale, bias = _weight_of(weight, weight_scale, bias, K, x2.device)
     with _on_device(x2.device) as stream:
-        q, scale, ld = _quantize(lib, x2, dtype, stream)
-        out = _int8_product(lib, q, ld, scale, x2.shape[0], weight, weight_scale, bias, relu, x.dtype, K, stream)
-    return out.view(*lead, out.shape[1])
+        out = torch.empty(lead + (N,), dtype=x.dtype, device=x2.device)
+        nbytes = lib.uhm_int8_linear_workspace_bytes(M, N, K)
+        ws = _workspace(nbytes, x2.device)
+        _lib.check_model(lib.uhm_int8_linear(x2.data_ptr(), dtype, _ld(x2), w.data_ptr(), w_ld, w_scale.data_ptr(), _ptr(bias),
+                                             out.data_ptr(), M, N, K, _lib.UHM_RELU if relu else 0, _ptr(ws), nbytes, stream),
+                         'uhm_int8_linear')
+    return out
