@@ -84,7 +84,7 @@ UHM_API int uhm_adam_clip_update(float* const* params, const void* const* grads,
                                  unsigned flags, const float* use_norm, float* norm, void* workspace, size_t workspace_bytes, uhm_stream_t stream);
 
 /* ---- products in 8-bit integers ---------------------------------------------------------------------------------------------
- * A matrix of rows in 8 bits: int8 [rows, K] with row stride ld (bytes; ld % 16 == 0, ld >= K), 16-byte aligned, and one f32
+ * A matrix of rows in 8 bits: int8 [rows, K] with row stride ld (bytes; ld % 16 == 0, K <= ld <= 2^23), 16-byte aligned, and one f32
  * scale per row; the value at (r, k) is q[r * ld + k] * scale[r].  Every row must be READABLE up to K rounded up to a multiple
  * of 16; what stands behind K does not matter.  Sums are exact in 32-bit integers: 1 <= K <= 131071 (131071 * 128^2 < 2^31).  */
 

@@ -60,50 +60,63 @@ __device__ __forceinline__ v4i load16(const int8_t* row, long long k, long long 
     return v;
 }
 
-template <int BM, int BN, int WM, int WN>      // WM x WN waves, each (BM / WM) x (BN / WN) outputs
-__global__ __launch_bounds__(WM * WN * 64) void int8_matmul_kernel(const int8_t* __restrict__ a, long long a_ld, const int8_t* __restrict__ b,
-                                                                   long long b_ld, int M, int N, int K, int tiles_per_split,
-                                                                   int* __restrict__ sums, const Epilogue e) {
-    constexpr int THREADS = WM * WN * 64, TM = BM / WM / 32, TN = BN / WN / 32;
-    constexpr int LA = BM * (BK / 16) / THREADS, LB = BN * (BK / 16) / THREADS;   // 16-byte chunks a thread stages
-    static_assert(LA >= 1 && LB >= 1 && LA * THREADS == BM * 8 && LB * THREADS == BN * 8, "staging");
-    __shared__ v4i sa[2][BM * 8], sb[2][BN * 8];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
-    const long long m0 = (long long)blockIdx.y * BM, n0 = (long long)blockIdx.x * BN;
-    const int ktiles = (K + BK - 1) / BK;
-    const int t0 = blockIdx.z * tiles_per_split, t1 = min(t0 + tiles_per_split, ktiles);
+// Where a block works: its tile and its range of K.  Consecutive blocks go to the 8 XCDs in turn, each with an L2 of its own: the
+// blocks of one XCD take a contiguous run of (K range, groups of 4 tile rows, tile columns), so that they share what they read.
+struct Place { int m, n, z; };
+__device__ __forceinline__ Place place(int mt, int nt, int splits) {
+    const unsigned total = (unsigned)mt * nt * splits, q = total / 8, r = total % 8, xcd = blockIdx.x % 8;
+    unsigned i = xcd * q + min(xcd, r) + blockIdx.x / 8;
+    const unsigned z = i / ((unsigned)mt * nt);
+    i -= z * mt * nt;
+    const unsigned group = i / (4u * nt), rows = min(4u, mt - group * 4);
+    i -= group * 4 * nt;
+    return {(int)(group * 4 + i % rows), (int)(i / rows), (int)z};
+}
 
-    // this thread's chunks: rows behind the last one repeat it (their outputs are not written)
-    const int8_t* pa[LA];
-    const int8_t* pb[LB];
-    int at_a[LA], at_b[LB];
-    const int chunk = tid & 7;
+template <int N> __device__ __forceinline__ void wait_for_loads() {          // ... but the last N, and every LDS read
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
+}
+
+template <int BM, int BN, int WM, int WN, int STAGES>      // WM x WN waves, each (BM / WM) x (BN / WN) outputs
+__global__ __launch_bounds__(WM * WN * 64, 1) void int8_matmul_kernel(const int8_t* __restrict__ a, long long a_ld, const int8_t* __restrict__ b,
+                                                                      long long b_ld, int M, int N, int K, int mt, int nt, int splits,
+                                                                      int tiles_per_split, int* __restrict__ sums, const Epilogue e) {
+    constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+    constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;           // loads (8 rows of 128 bytes each) of a wave per tile
+    static_assert(LA >= 1 && LB >= 1 && LA * WAVES * 8 == BM && LB * WAVES * 8 == BN, "staging");
+    __shared__ v4i sa[STAGES][BM * 8], sb[STAGES][BN * 8];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+    const Place at = place(mt, nt, splits);
+    const long long m0 = (long long)at.m * BM, n0 = (long long)at.n * BN;
+    const int t0 = at.z * tiles_per_split, t1 = min(t0 + tiles_per_split, (K + BK - 1) / BK), whole = min(t1, K / BK);
+
+    // this lane's 16 bytes of each load: row lane / 8 of eight, the chunk that belongs at position lane % 8 of it; rows behind the
+    // last one repeat it (their outputs are not written)
+    const int8_t* const base_a = a + m0 * a_ld;
+    const int8_t* const base_b = b + n0 * b_ld;
+    const unsigned chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+    unsigned row_a[LA], row_b[LB];                                        // (256 rows of at most MAX_LD: 32 bits)
 #pragma unroll
-    for (int i = 0; i < LA; ++i) {
-        const int r = (tid >> 3) + i * (THREADS / 8);
-        pa[i] = a + min(m0 + r, (long long)M - 1) * a_ld;
-        at_a[i] = r * 8 + (chunk ^ (r & 7));
-    }
+    for (int i = 0; i < LA; ++i) row_a[i] = (unsigned)min((long long)(i * WAVES + wave) * 8 + (lane >> 3), M - 1 - m0) * (unsigned)a_ld;
 #pragma unroll
-    for (int i = 0; i < LB; ++i) {
-        const int r = (tid >> 3) + i * (THREADS / 8);
-        pb[i] = b + min(n0 + r, (long long)N - 1) * b_ld;
-        at_b[i] = r * 8 + (chunk ^ (r & 7));
-    }
-    v4i ra[LA], rb[LB];
-    auto load = [&](int t) {
-        const long long k = (long long)t * BK + chunk * 16;
-#pragma unroll
-        for (int i = 0; i < LA; ++i) ra[i] = load16(pa[i], k, K, true);
-#pragma unroll
-        for (int i = 0; i < LB; ++i) rb[i] = load16(pb[i], k, K, false);
+    for (int i = 0; i < LB; ++i) row_b[i] = (unsigned)min((long long)(i * WAVES + wave) * 8 + (lane >> 3), N - 1 - n0) * (unsigned)b_ld;
+    auto to_lds = [](const int8_t* p, v4i* s) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)s, 16, 0, 0);
     };
-    auto store = [&](int buf) {
+    auto fetch = [&](int t, int buf) {
+        const int k = t * BK;
+        if (t < whole) {
 #pragma unroll
-        for (int i = 0; i < LA; ++i) sa[buf][at_a[i]] = ra[i];
+            for (int i = 0; i < LA; ++i) to_lds(base_a + k + (row_a[i] + chunk), &sa[buf][(i * WAVES + wave) * 64]);
 #pragma unroll
-        for (int i = 0; i < LB; ++i) sb[buf][at_b[i]] = rb[i];
+            for (int i = 0; i < LB; ++i) to_lds(base_b + k + (row_b[i] + chunk), &sb[buf][(i * WAVES + wave) * 64]);
+        } else {                                                  // the tile that K ends in, through registers: zeros behind K
+#pragma unroll
+            for (int i = 0; i < LA; ++i) sa[buf][(i * WAVES + wave) * 64 + lane] = load16(base_a + row_a[i], k + chunk, K, true);
+#pragma unroll
+            for (int i = 0; i < LB; ++i) sb[buf][(i * WAVES + wave) * 64 + lane] = load16(base_b + row_b[i], k + chunk, K, false);
+        }
     };
 
     v16i acc[TM][TN];
@@ -112,54 +125,73 @@ __global__ __launch_bounds__(WM * WN * 64) void int8_matmul_kernel(const int8_t*
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = v16i{};
 
-    if (t0 < t1) {
-        load(t0);
-        store(0);
-        if (t0 + 1 < t1) load(t0 + 1);
-        __syncthreads();
-        const int row = lane & 31, half = lane >> 5;
-        for (int t = t0; t < t1; ++t) {
-            const int buf = (t - t0) & 1;
 #pragma unroll
-            for (int s = 0; s < BK / 32; ++s) {
-                v4i fa[TM], fb[TN];
-                const int c = 2 * s + half;
+    for (int i = 0; i < STAGES - 1; ++i)
+        if (t0 + i < t1) fetch(t0 + i, i);
+    const int row = lane & 31, half = lane >> 5;
+    int buf = 0;
+    for (int t = t0; t < t1; ++t) {
+        // tile t is in LDS for every wave, and none still reads the buffer that is filled next
+        if (t + STAGES - 2 < whole) wait_for_loads<(LA + LB) * (STAGES - 2)>();
+        else wait_for_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (t + STAGES - 1 < t1) fetch(t + STAGES - 1, buf == 0 ? STAGES - 1 : buf - 1);
+        // the operands of step s + 1 are read while the matrix instructions of step s run, and no earlier: two sets of registers
+        v4i fa[2][TM], fb[2][TN];
+        auto read = [&](int s) {
+            const int c = (2 * s + half) ^ (row & 7);
 #pragma unroll
-                for (int i = 0; i < TM; ++i) { const int r = wm + i * 32 + row; fa[i] = sa[buf][r * 8 + (c ^ (r & 7))]; }
+            for (int i = 0; i < TM; ++i) fa[s & 1][i] = sa[buf][(wm + i * 32 + row) * 8 + c];
 #pragma unroll
-                for (int j = 0; j < TN; ++j) { const int r = wn + j * 32 + row; fb[j] = sb[buf][r * 8 + (c ^ (r & 7))]; }
+            for (int j = 0; j < TN; ++j) fb[s & 1][j] = sb[buf][(wn + j * 32 + row) * 8 + c];
+        };
+        read(0);
 #pragma unroll
-                for (int i = 0; i < TM; ++i)
+        for (int s = 0; s < BK / 32; ++s) {
+            if (s + 1 < BK / 32) read(s + 1);
 #pragma unroll
-                    for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fb[j], acc[i][j], 0, 0, 0);
-            }
-            if (t + 1 < t1) {
-                store(buf ^ 1);                                  // everyone left this buffer before the last barrier
-                if (t + 2 < t1) load(t + 2);
-            }
-            __syncthreads();
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[s & 1][i], fb[s & 1][j], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        buf = buf + 1 == STAGES ? 0 : buf + 1;
     }
 
     // D of a 32 x 32 tile: lane l, register i hold row 8 (i / 4) + 4 (l / 32) + i % 4, column l % 32
-    const int col = lane & 31, r4 = (lane >> 5) * 4;
-    const bool split = sums != nullptr;
-    int* part = sums + (size_t)blockIdx.z * M * N;
+    auto each = [&](auto out) {
+        float sbn[TN], bias[TN];
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const long long n = n0 + wn + j * 32 + col;
-        if (n >= N) continue;
-        const float sbn = split ? 0.f : e.b_scale[n], bias = split || !e.bias ? 0.f : e.bias[n];
+        for (int j = 0; j < TN; ++j) {
+            const long long n = min(n0 + wn + j * 32 + row, (long long)N - 1);
+            sbn[j] = sums ? 0.f : e.b_scale[n];
+            bias[j] = sums || !e.bias ? 0.f : e.bias[n];
+        }
+        int m = (int)m0 + wm + half * 4;
+        size_t at = (size_t)m * N + n0 + wn + row;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-                const long long m = m0 + wm + i * 32 + 8 * (k >> 2) + r4 + (k & 3);
-                if (m >= M) continue;
-                const size_t at = (size_t)m * N + n;
-                if (split) part[at] = acc[i][j][k];
-                else put(e.out, e.dtype, at, finish(acc[i][j][k], e.a_scale[m], sbn, bias, e.relu));
+                asm volatile("" : "+v"(m), "+v"(at));            // (one row's address at a time: all of them at once would spill)
+                if (m < M) {
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+                        if (n0 + wn + j * 32 + row < N) out(at + j * 32, acc[i][j][k], m, sbn[j], bias[j]);
+                }
+                const int step = (k & 3) == 3 ? 5 : 1;
+                m += step;
+                at += step * (size_t)N;
             }
+    };
+    if (sums) {
+        int* part = sums + (size_t)at.z * M * N;
+        each([&](size_t at, int v, int, float, float) { part[at] = v; });
+    } else if (e.dtype == UHM_F32) {
+        each([&](size_t at, int v, int m, float sbn, float bias) { ((float*)e.out)[at] = finish(v, e.a_scale[m], sbn, bias, e.relu); });
+    } else {
+        each([&](size_t at, int v, int m, float sbn, float bias) { put(e.out, e.dtype, at, finish(v, e.a_scale[m], sbn, bias, e.relu)); });
     }
 }
 
@@ -375,21 +407,23 @@ __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x,
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 constexpr long long MAX_K = 131071, MAX_DIM = 0x7fffffffLL - 512;
+constexpr long long MAX_LD = 1LL << 23;     // 256 rows of it are indexed in 32 bits
 constexpr long long FEW = 4;               // tokens up to which the weight is read by int8_few_kernel
 
 struct Plan { int bm, bn, splits, tiles_per_split; };
 
-// v1 rule: the tile follows M; K is split until about 512 blocks run, each keeping at least 4 tiles of K
 inline Plan plan_of(long long M, long long N, long long K) {
+    const auto tiles_of = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
     Plan p;
-    if (M <= 32) { p.bm = 32; p.bn = 128; }
-    else if (M <= 64) { p.bm = 64; p.bn = 128; }
-    else { p.bm = 128; p.bn = 128; }
-    if (((M + 255) / 256) * ((N + 255) / 256) >= 200) p.bm = p.bn = 256;
-    const long long tiles = ((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn), kt = (K + BK - 1) / BK;
-    long long s = 1;
-    if (tiles < 256) s = 512 / tiles;
-    if (s > kt / 4) s = kt / 4;
+    long long most;                            // splits: past these the partial sums cost more than the blocks they add bring
+    if (M <= 32) { p.bm = 32; p.bn = 128; most = 32; }
+    else if (tiles_of(256, 256) >= 200) { p.bm = p.bn = 256; most = 1; }
+    else if (tiles_of(128, 128) >= 200) { p.bm = p.bn = 128; most = 1; }
+    else { p.bm = p.bn = 64; most = 16; }
+    const long long tiles = tiles_of(p.bm, p.bn), kt = (K + BK - 1) / BK;
+    long long s = tiles < 256 ? 512 / tiles : 1;
+    if (s > most) s = most;
+    if (s > kt / 8) s = kt / 8;                // at least 8 tiles of K each: a block's first loads take as long as several tiles
     if (s < 1) s = 1;
     p.tiles_per_split = (int)((kt + s - 1) / s);
     p.splits = (int)((kt + p.tiles_per_split - 1) / p.tiles_per_split);
@@ -399,8 +433,8 @@ inline Plan plan_of(long long M, long long N, long long K) {
 int check_product(long long M, long long N, long long K) {
     if (M < 0 || N < 0 || K < 1) return UHM_E_SHAPE;
     if (K > MAX_K || M > MAX_DIM || N > MAX_DIM) return UHM_E_TOO_LARGE;
-    // grid: blocks along M in gridDim.y, sizes of the output in 64 bits
-    if ((M + 31) / 32 > 65535) return UHM_E_TOO_LARGE;
+    // the grid is a line of blocks: at most 2^23 tiles (K is only split where they are few)
+    if (((M + 31) / 32) * ((N + 63) / 64) > (1LL << 23)) return UHM_E_TOO_LARGE;
     return 0;
 }
 
@@ -409,6 +443,7 @@ int check_operands(const void* x, long long x_ld, const int8_t* b, long long b_l
                    int out_dtype, long long M, long long N, long long K, unsigned flags) {
     if (int err = check_product(M, N, K)) return err;
     if (x_ld < K || b_ld < K) return UHM_E_SHAPE;
+    if (N > 1 && b_ld > MAX_LD) return UHM_E_TOO_LARGE;
     if (out_dtype < UHM_F32 || out_dtype > UHM_F16) return UHM_E_DTYPE;
     if (flags & ~UHM_RELU) return UHM_E_VALUE;
     if (M == 0 || N == 0) return 0;
@@ -461,15 +496,16 @@ int product(const int8_t* a, long long a_ld, const int8_t* b, long long b_ld, lo
     if (M <= 2) return launch_few<2, -1>(a, a_ld, 1, b, b_ld, (int)M, (int)N, (int)K, e, s);
     if (M <= FEW) return launch_few<4, -1>(a, a_ld, 1, b, b_ld, (int)M, (int)N, (int)K, e, s);
     const Plan p = plan_of(M, N, K);
-    const dim3 grid((unsigned)((N + p.bn - 1) / p.bn), (unsigned)((M + p.bm - 1) / p.bm), (unsigned)p.splits);
+    const int mt = (int)((M + p.bm - 1) / p.bm), nt = (int)((N + p.bn - 1) / p.bn);
     if (p.splits == 1) sums = nullptr;
     auto launch = [&](auto kernel, int threads) {
-        hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, a, a_ld, b, b_ld, (int)M, (int)N, (int)K, p.tiles_per_split, sums, e);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)mt * nt * p.splits), dim3(threads), 0, s, a, a_ld, b, b_ld, (int)M, (int)N, (int)K, mt, nt, p.splits,
+                           p.tiles_per_split, sums, e);
     };
-    if (p.bm == 32) launch(int8_matmul_kernel<32, 128, 1, 4>, 256);
-    else if (p.bm == 64) launch(int8_matmul_kernel<64, 128, 2, 2>, 256);
-    else if (p.bm == 128) launch(int8_matmul_kernel<128, 128, 2, 2>, 256);
-    else launch(int8_matmul_kernel<256, 256, 2, 4>, 512);
+    if (p.bm == 32) launch(int8_matmul_kernel<32, 128, 1, 4, 4>, 256);
+    else if (p.bm == 64) launch(int8_matmul_kernel<64, 64, 2, 2, 5>, 256);
+    else if (p.bm == 128) launch(int8_matmul_kernel<128, 128, 2, 2, 4>, 256);
+    else launch(int8_matmul_kernel<256, 256, 2, 4, 2>, 512);
     if (int err = (int)hipGetLastError()) return err;
     if (p.splits > 1) {
         const long long blocks = (M * N + 255) / 256;
@@ -531,6 +567,7 @@ extern "C" int uhm_int8_matmul(const int8_t* a, long long a_ld, const float* a_s
     if (int err = check_operands(a, a_ld, b, b_ld, b_scale, bias, out, out_dtype, M, N, K, flags)) return err;
     if (M == 0 || N == 0) return 0;
     if (!a_scale) return UHM_E_NULL;
+    if (M > 1 && a_ld > MAX_LD) return UHM_E_TOO_LARGE;
     if ((((uintptr_t)a | (uintptr_t)a_ld) & 15) || ((uintptr_t)a_scale & 3)) return UHM_E_ALIGN;
     if (int err = check_space(workspace, workspace_bytes, sums_bytes(M, N, K))) return err;
     const Epilogue e = {a_scale, b_scale, bias, out, out_dtype, (flags & UHM_RELU) ? 1 : 0};
