@@ -68,6 +68,7 @@ SIGNATURES = {
 
 # ---- include/uh_model_ops.h ------------------------------------------------------------------------------------------
 MODEL_OPS_PATH = os.path.join(HERE, 'lib', 'libuh_model_ops.so')
+TORCH_OPS_PATH = os.path.join(HERE, 'lib', '_uhm_torch.so')           # csrc/uhm_torch.cpp: the same on torch tensors
 UHM_ABI_VERSION = 1
 UHM_F32, UHM_BF16, UHM_F16 = 0, 1, 2
 UHM_SKIP_NONFINITE = 1
@@ -92,6 +93,7 @@ MODEL_OPS_SIGNATURES = {
 
 _lib = None
 _model_ops = None
+_torch_ops = None
 
 
 class UHError(RuntimeError):
@@ -136,9 +138,25 @@ def load_model_ops():
     return lib
 
 
-def check_model(code, what):
-    if code != 0:
-        raise UHError('%s failed: %s (code %d)' % (what, load_model_ops().uhm_error_string(code).decode(), code))
+def load_torch_ops():
+    """Import the module _uhm_torch (once): the operators of libuh_model_ops.so on torch tensors."""
+    global _torch_ops
+    if _torch_ops is not None:
+        return _torch_ops
+    import importlib.machinery
+    import importlib.util
+    import torch  # noqa: F401  (its libraries first)
+    load_model_ops()
+    if not os.path.exists(TORCH_OPS_PATH):
+        raise UHError('%s not found -- run `python -c "import __graft_entry__ as g; g.build()"`' % TORCH_OPS_PATH)
+    loader = importlib.machinery.ExtensionFileLoader('_uhm_torch', TORCH_OPS_PATH)
+    mod = importlib.util.module_from_spec(importlib.util.spec_from_loader('_uhm_torch', loader))
+    loader.exec_module(mod)
+    if mod.abi_version() != UHM_ABI_VERSION:
+        raise UHError('ABI version mismatch: %s is built for %d, binding %d' % (TORCH_OPS_PATH, mod.abi_version(), UHM_ABI_VERSION))
+    mod.set_error(UHError)
+    _torch_ops = mod
+    return mod
 
 
 def check(code, what):

@@ -21,6 +21,8 @@ HEADERS = ['uh_device.h', 'uh_host.h', os.path.join('..', '..', 'include', 'uh_h
 MODEL_OPS_LIB = os.path.join(LIBDIR, 'libuh_model_ops.so')
 MODEL_OPS_SOURCES = ['uhm_multi.hip', 'uhm_int8.hip']
 MODEL_OPS_HEADERS = [os.path.join('..', '..', 'include', 'uh_model_ops.h')]
+TORCH_OPS_LIB = os.path.join(LIBDIR, '_uhm_torch.so')
+TORCH_OPS_SOURCES = ['uhm_torch.cpp']
 # `-packed-fp32-ops`: no v_pk_{add,mul,fma}_f32 anywhere -- some of their forms have given wrong results now and then on gfx950.
 # The scalar forms round the same, and every kernel keeps its register count (the warp and patch kernels lose 224 packed
 # instructions, the others had none).  hipcc's host pass warns that it does not know the feature: harmless.
@@ -43,18 +45,19 @@ def find_hipcc():
     raise RuntimeError('hipcc not found: cannot build libuh_hotpath.so')
 
 
-def _build(lib, sources, headers, force, verbose):
+def _build(lib, sources, headers, force, verbose, command=None):
     os.makedirs(LIBDIR, exist_ok=True)
     stamp = lib + '.sha256'
     fp = _fingerprint(sources + headers)
     if not force and os.path.exists(lib) and os.path.exists(stamp) and open(stamp).read().strip() == fp:
         return lib
-    cmd = [find_hipcc()] + FLAGS + [os.path.join(CSRC, s) for s in sources] + ['-o', lib + '.tmp']
+    before, after = command() if command else ([find_hipcc()] + FLAGS, [])
+    cmd = before + [os.path.join(CSRC, s) for s in sources] + after + ['-o', lib + '.tmp']
     if verbose:
         print(' '.join(cmd))
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError('hipcc failed:\n' + res.stdout + res.stderr)
+        raise RuntimeError('%s failed:\n' % os.path.basename(cmd[0]) + res.stdout + res.stderr)
     os.replace(lib + '.tmp', lib)
     with open(stamp, 'w') as fh:
         fh.write(fp)
@@ -67,8 +70,27 @@ def build_library(force=False, verbose=False):
 
 
 def build_model_ops(force=False, verbose=False):
-    """Compile csrc/uhm_*.hip -> lib/libuh_model_ops.so.  Returns the library path."""
-    return _build(MODEL_OPS_LIB, MODEL_OPS_SOURCES, MODEL_OPS_HEADERS, force, verbose)
+    """Compile csrc/uhm_*.hip -> lib/libuh_model_ops.so, and csrc/uhm_torch.cpp -> lib/_uhm_torch.so on top of it.  Returns the
+    library path."""
+    lib = _build(MODEL_OPS_LIB, MODEL_OPS_SOURCES, MODEL_OPS_HEADERS, force, verbose)
+    _build(TORCH_OPS_LIB, TORCH_OPS_SOURCES, MODEL_OPS_HEADERS, force, verbose, torch_command)
+    return lib
+
+
+def torch_command():
+    """The host compiler's command for a Python module on torch's and this package's libraries."""
+    import sysconfig
+    import torch
+    base = os.path.dirname(torch.__file__)
+    cxx = os.environ.get('CXX') or shutil.which('g++') or shutil.which('c++')
+    if not cxx:
+        raise RuntimeError('no C++ compiler: cannot build _uhm_torch.so')
+    includes = [os.path.join(base, 'include'), os.path.join(base, 'include', 'torch', 'csrc', 'api', 'include'),
+                os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(find_hipcc()))), 'include'), sysconfig.get_paths()['include']]
+    return ([cxx, '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
+             '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch._C._GLIBCXX_USE_CXX11_ABI] + ['-I' + i for i in includes],
+            ['-L' + LIBDIR, '-luh_model_ops', '-L' + os.path.join(base, 'lib'), '-lc10', '-lc10_hip', '-ltorch_cpu', '-ltorch', '-ltorch_python',
+             '-Wl,-rpath,$ORIGIN'])
 
 
 def kernel_resources(force=False, sources=None, headers=None):

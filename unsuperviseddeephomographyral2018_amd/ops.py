@@ -18,7 +18,6 @@ Around the regressor (include/uh_model_ops.h; no counterpart in the reference):
   quantize_rows, int8_matmul, int8_linear                     products in 8-bit integers for the fully connected head in evaluation
 """
 import ctypes as C
-from array import array
 
 import numpy as np
 import torch
@@ -723,320 +722,57 @@ def conv_bias_relu_pool(x, weight, bias, padding=1):
 
 
 # ------------------------------------------------------------------------------------------------
-# Lists of tensors (include/uh_model_ops.h): the optimizer's side of a training step.
-_UHM_DTYPES = {torch.float32: _lib.UHM_F32, torch.bfloat16: _lib.UHM_BF16, torch.float16: _lib.UHM_F16}
-
-
-class _on_device(object):
-    """The tensors' device as the current one for the length of a call, and its current stream."""
-
-    def __init__(self, device):
-        self.device = device
-        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
-def _check_list(tensors, name, dtypes=_UHM_DTYPES):
-    tensors = list(tensors)
-    if not tensors:
-        raise _lib.UHError('%s: at least one tensor is needed' % name)
-    device = tensors[0].device if isinstance(tensors[0], torch.Tensor) else None
-    for t in tensors:
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.layout is not torch.strided:
-            raise _lib.UHError('%s must be dense tensors on the HIP device (got %s); there is no CPU fallback'
-                               % (name, getattr(t, 'device', type(t))))
-        if t.dtype not in dtypes:
-            raise _lib.UHError('%s: %s is not supported (%s)' % (name, t.dtype, ', '.join(str(d) for d in dtypes)))
-        if t.device != device:
-            raise _lib.UHError('%s: tensors on several devices (%s, %s)' % (name, device, t.device))
-    return tensors, device
-
-
-def _no_grad_wanted(tensors, name):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t.requires_grad:
-                raise _lib.UHError('%s has no gradient: pass detached tensors or call it under torch.no_grad()' % name)
-
-
-def _is_dense(t):
-    """Whether the elements fill one piece of memory without gaps, in the usual orders."""
-    return t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last)) \
-        or (t.dim() == 2 and t.t().is_contiguous())
-
-
-def _pointers(tensors):
-    return array('Q', [t.data_ptr() for t in tensors])
-
-
-def _addr(a):
-    return a.buffer_info()[0]
-
-
-def _lengths_and_types(tensors):
-    return array('q', [t.numel() for t in tensors]), array('i', [_UHM_DTYPES[t.dtype] for t in tensors])
-
-
-def _multi_workspace(lib, count, device):
-    nbytes = lib.uhm_multi_workspace_bytes(count)
-    return torch.empty((nbytes // 8,), dtype=torch.float64, device=device), nbytes
-
-
-def _clip_value(clip_norm, name):
-    clip_norm = float(clip_norm)
-    if not clip_norm > 0.0:
-        raise _lib.UHError('%s: clip_norm must be > 0 (got %s)' % (name, clip_norm))
-    return clip_norm
-
-
-def _given_norm(use_norm, device, name):
-    if use_norm is None:
-        return None
-    use_norm = _f32(use_norm, 'use_norm')
-    if use_norm.numel() != 1 or use_norm.device != device:
-        raise _lib.UHError('%s: use_norm must be one float32 value on %s' % (name, device))
-    return use_norm
-
-
+# Lists of tensors (include/uh_model_ops.h through csrc/uhm_torch.cpp): the optimizer's side of a training step.
 def global_norm(tensors):
     """sqrt of the sum of all squares over a list of float32 / bfloat16 / float16 tensors (mixed, of any shapes and dense or
     strided layouts, empty ones among them), as tf.global_norm -> float32 scalar on their device.  Squares are added in f64 in a
     fixed order: the result is the same on every call, and finite lists neither overflow nor vanish on the way.  No gradient."""
-    lib = _lib.load_model_ops()
-    tensors, device = _check_list(tensors, 'tensors')
-    _no_grad_wanted(tensors, 'global_norm')
-    tensors = [t if _is_dense(t) else t.contiguous() for t in tensors]
-    numel, dtypes = _lengths_and_types(tensors)
-    ptrs = _pointers(tensors)
-    with _on_device(device) as stream:
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        ws, nbytes = _multi_workspace(lib, len(tensors), device)
-        _lib.check_model(lib.uhm_global_norm(_addr(ptrs), _addr(numel), _addr(dtypes), len(tensors), norm.data_ptr(), ws.data_ptr(),
-                                             nbytes, stream), 'uhm_global_norm')
-    return norm
-
-
-def _clip(tensors, out, clip_norm, use_norm, device, name):
-    lib = _lib.load_model_ops()
-    numel, dtypes = _lengths_and_types(tensors)
-    ptrs = _pointers(tensors)
-    outs = ptrs if out is tensors else _pointers(out)
-    with _on_device(device) as stream:
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        ws, nbytes = _multi_workspace(lib, len(tensors), device) if use_norm is None else (None, 0)
-        _lib.check_model(lib.uhm_clip_by_global_norm(_addr(ptrs), _addr(outs), _addr(numel), _addr(dtypes), len(tensors), clip_norm,
-                                                     _ptr(use_norm), norm.data_ptr(), _ptr(ws), nbytes, stream), name)
-    return norm
+    return _lib.load_torch_ops().global_norm(tensors)
 
 
 def clip_by_global_norm(tensors, clip_norm, use_norm=None):
     """tf.clip_by_global_norm: -> (list of t * clip_norm / max(norm, clip_norm), norm), in each tensor's type.  A norm that is not
     finite makes every value NaN.  use_norm: a norm computed before (float32 scalar on the device).  No gradient."""
-    name = 'clip_by_global_norm'
-    clip_norm = _clip_value(clip_norm, name)
-    tensors, device = _check_list(tensors, 'tensors')
-    _no_grad_wanted(tensors, name)
-    use_norm = _given_norm(use_norm, device, name)
-    tensors = [t if _is_dense(t) else t.contiguous() for t in tensors]
-    out = [torch.empty_like(t) for t in tensors]
-    return out, _clip(tensors, out, clip_norm, use_norm, device, name)
+    return _lib.load_torch_ops().clip_by_global_norm(tensors, clip_norm, use_norm)
 
 
 def clip_by_global_norm_(tensors, clip_norm, use_norm=None):
-    """clip_by_global_norm in place -> norm.  When nothing has to be clipped, nothing is written.  A tensor that is given twice, or
-    whose elements overlap (expanded), is refused.  Can be captured into a hipGraph."""
-    name = 'clip_by_global_norm_'
-    clip_norm = _clip_value(clip_norm, name)
-    tensors, device = _check_list(tensors, 'tensors')
-    _no_grad_wanted(tensors, name)
-    use_norm = _given_norm(use_norm, device, name)
-    work = []
-    for t in tensors:
-        if _is_dense(t):
-            work.append(t)
-        else:                                # slices of something larger: clipped in a copy
-            if any(st == 0 and n > 1 for n, st in zip(t.shape, t.stride())):
-                raise _lib.UHError('%s: an expanded tensor cannot be written in place' % name)
-            work.append(t.contiguous())
-    norm = _clip(work, work, clip_norm, use_norm, device, name)
-    with torch.no_grad():
-        for t, w in zip(tensors, work):
-            if w is not t:
-                t.copy_(w)
-    torch.autograd.graph.increment_version(tensors)
-    return norm
+    """clip_by_global_norm in place -> norm.  When nothing has to be clipped, nothing is written.  A tensor that is given twice,
+    tensors that overlap, and expanded ones are refused.  Can be captured into a hipGraph."""
+    return _lib.load_torch_ops().clip_by_global_norm_(tensors, clip_norm, use_norm)
 
 
 def adam_clip_update_(params, grads, exp_avgs, exp_avg_sqs, lr, beta1=0.9, beta2=0.999, eps=1e-8, step=1, clip_norm=1.0,
                       use_norm=None, skip_nonfinite=False):
     """One Adam step (torch.optim.Adam's rule, no weight decay) with the gradients clipped by their global norm on the way
     -> norm.  params, exp_avgs, exp_avg_sqs: float32, updated in place; grads: float32 / bfloat16 / float16, only read; the four
-    lists in the same order, shapes and (dense) layouts.  step counts from 1.  clip_norm may be inf (the norm is then only told).
-    use_norm: a norm computed before, for lists that are part of a larger one.  A norm that is not finite makes params and moments
-    NaN, or with skip_nonfinite leaves them as they are.  Can be captured into a hipGraph (with the scalars of that call)."""
-    name = 'adam_clip_update_'
-    lib = _lib.load_model_ops()
-    clip_norm = _clip_value(clip_norm, name)
-    params, device = _check_list(params, 'params', (torch.float32,))
-    grads, gdev = _check_list(grads, 'grads')
-    exp_avgs, mdev = _check_list(exp_avgs, 'exp_avgs', (torch.float32,))
-    exp_avg_sqs, vdev = _check_list(exp_avg_sqs, 'exp_avg_sqs', (torch.float32,))
-    if not (len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs)):
-        raise _lib.UHError('%s: lists of %d, %d, %d and %d tensors' % (name, len(params), len(grads), len(exp_avgs), len(exp_avg_sqs)))
-    if not (device == gdev == mdev == vdev):
-        raise _lib.UHError('%s: lists on several devices' % name)
-    use_norm = _given_norm(use_norm, device, name)
-    kept = []
-    for p, g, m, v in zip(params, grads, exp_avgs, exp_avg_sqs):
-        if not (p.shape == g.shape == m.shape == v.shape):
-            raise _lib.UHError('%s: shapes %s, %s, %s, %s' % (name, tuple(p.shape), tuple(g.shape), tuple(m.shape), tuple(v.shape)))
-        st = p.stride()
-        if not _is_dense(p) or m.stride() != st or v.stride() != st:
-            raise _lib.UHError('%s: params and moments must be dense and laid out alike' % name)
-        kept.append(g if g.stride() == st else torch.empty_like(p, dtype=g.dtype).copy_(g.detach()))
-    lists = [_pointers(x) for x in (params, kept, exp_avgs, exp_avg_sqs)]
-    numel, dtypes = _lengths_and_types(kept)
-    with _on_device(device) as stream:
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        ws, nbytes = _multi_workspace(lib, len(params), device) if use_norm is None else (None, 0)
-        _lib.check_model(lib.uhm_adam_clip_update(*[_addr(x) for x in lists], _addr(numel), _addr(dtypes), len(params), lr, beta1,
-                                                  beta2, eps, int(step), clip_norm,
-                                                  _lib.UHM_SKIP_NONFINITE if skip_nonfinite else 0, _ptr(use_norm), norm.data_ptr(),
-                                                  _ptr(ws), nbytes, stream), name)
-    torch.autograd.graph.increment_version(params + exp_avgs + exp_avg_sqs)
-    return norm
+    lists in the same order and shapes; params and moments dense and laid out alike.  step counts from 1.  clip_norm may be inf
+    (the norm is then only told).  use_norm: a norm computed before, for lists that are part of a larger one.  A norm that is not
+    finite makes params and moments NaN, or with skip_nonfinite leaves them as they are.  Can be captured into a hipGraph (with the
+    scalars of that call)."""
+    return _lib.load_torch_ops().adam_clip_update_(params, grads, exp_avgs, exp_avg_sqs, lr, beta1, beta2, eps, int(step), clip_norm, use_norm,
+                                                   bool(skip_nonfinite))
 
 
 # ------------------------------------------------------------------------------------------------
-# Products in 8-bit integers (include/uh_model_ops.h): rows of values with one scale each.
-def _rows_of(x, name):
-    """x [..., K] as rows: (2-D tensor whose rows are contiguous and do not overlap, leading shape, K)."""
-    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.layout is not torch.strided:
-        raise _lib.UHError('%s must be a tensor on the HIP device (got %s); there is no CPU fallback'
-                           % (name, getattr(x, 'device', type(x))))
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise _lib.UHError('%s must be [..., K] with K >= 1 (got %s)' % (name, tuple(x.shape)))
-    K = x.shape[-1]
-    x2 = x if x.dim() == 2 else x.reshape(-1, K) if x.numel() else x.new_empty((0, K))
-    if x2.shape[0] and (x2.stride(1) != 1 and K > 1 or x2.shape[0] > 1 and x2.stride(0) < K):
-        x2 = x2.contiguous()
-    return x2, x.shape[:-1], K
-
-
-def _ld(x2):
-    return max(x2.stride(0), x2.shape[1])           # (a single row may carry any stride)
-
-
-def _quantize(lib, x2, dtype, stream):
-    rows, K = x2.shape
-    ld = -(-K // 128) * 128                          # rows start on 128 bytes
-    q = torch.empty((rows, ld), dtype=torch.int8, device=x2.device)
-    scale = torch.empty((rows,), dtype=torch.float32, device=x2.device)
-    _lib.check_model(lib.uhm_quantize_rows(x2.data_ptr(), dtype, _ld(x2), q.data_ptr(), ld, scale.data_ptr(), rows, K, stream),
-                     'uhm_quantize_rows')
-    return q, scale, ld
-
-
-def _float_rows(x, name):
-    x2, lead, K = _rows_of(x, name)
-    if x.dtype not in _UHM_DTYPES:
-        raise _lib.UHError('%s: %s is not supported (float32, bfloat16, float16)' % (name, x.dtype))
-    return x2, lead, K, _UHM_DTYPES[x.dtype]
-
-
+# Products in 8-bit integers (include/uh_model_ops.h through csrc/uhm_torch.cpp): rows of values with one scale each.
 def quantize_rows(x):
     """Rows of x [..., K] in 8 bits, one scale each -> (q int8 [..., K], scale float32 [...]); q * scale stands for x:
     scale = max |x| / 127 and q = x * (127 / max |x|) rounded to nearest even.  Used for the tokens (rows of activations) and for
     the channels (rows of a weight [N, K]) of int8_matmul; rows of q start on 128 bytes.  A row that holds an infinity or NaN gets
     a NaN scale: every product with it is NaN.  No gradient."""
-    lib = _lib.load_model_ops()
-    x2, lead, K, dtype = _float_rows(x, 'x')
-    _no_grad_wanted((x,), 'quantize_rows')
-    with _on_device(x2.device) as stream:
-        q, scale, ld = _quantize(lib, x2, dtype, stream)
-    return q.view(*lead, ld)[..., :K], scale.view(lead)
-
-
-def _int8_rows(q, name):
-    """(tensor that owns the memory, rows, K, row stride) as uhm_int8_matmul takes them: aligned rows, each readable up to the next
-    multiple of 16.  quantize_rows gives such rows; others are copied."""
-    q2, lead, K = _rows_of(q, name)
-    if q.dtype != torch.int8:
-        raise _lib.UHError('%s must be int8 (got %s)' % (name, q.dtype))
-    rows = q2.shape[0]
-    ld = _ld(q2)
-    if rows == 1:
-        ld = -(-ld // 16) * 16
-    if rows and (ld % 16 or q2.data_ptr() % 16 or
-                 q2.untyped_storage().nbytes() - q2.storage_offset() < (rows - 1) * ld + -(-K // 16) * 16):
-        ld = -(-K // 128) * 128
-        q2 = torch.zeros((rows, ld), dtype=torch.int8, device=q.device)[:, :K].copy_(q2)
-    return q2, lead, rows, K, ld
-
-
-def _row_scales(scale, rows, device, name):
-    scale = _f32(scale, name)
-    if scale.numel() != rows or scale.device != device:
-        raise _lib.UHError('%s must hold %d values on %s' % (name, rows, device))
-    return scale
-
-
-def _weight_of(weight, weight_scale, bias, K, device):
-    w2, lead, N, wK, w_ld = _int8_rows(weight, 'weight')
-    if len(lead) != 1 or wK != K or w2.device != device:
-        raise _lib.UHError('weight must be int8 [N, %d] on %s (got %s on %s)' % (K, device, tuple(weight.shape), weight.device))
-    if bias is not None:
-        bias = _row_scales(bias, N, device, 'bias')
-    return w2, w_ld, N, _row_scales(weight_scale, N, device, 'weight_scale'), bias
-
-
-def _workspace(nbytes, device):
-    return torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
+    return _lib.load_torch_ops().quantize_rows(x)
 
 
 def int8_matmul(x, x_scale, weight, weight_scale, bias=None, relu=False, out_dtype=torch.float32):
     """act((x . weight^T) * x_scale * weight_scale + bias): x int8 [..., K] with one scale per token (x_scale [...]), weight
     int8 [N, K] with one per channel (weight_scale [N]), bias float32 [N] or None, act = relu or nothing -> [..., N] in out_dtype
     (float32, bfloat16, float16).  The sums are exact (K <= 131071).  No gradient."""
-    lib = _lib.load_model_ops()
-    if out_dtype not in _UHM_DTYPES:
-        raise _lib.UHError('int8_matmul: out_dtype %s is not supported' % (out_dtype,))
-    _no_grad_wanted([t for t in (x_scale, weight_scale, bias) if isinstance(t, torch.Tensor)], 'int8_matmul')
-    x2, lead, M, K, x_ld = _int8_rows(x, 'x')
-    x_scale = _row_scales(x_scale, M, x2.device, 'x_scale')
-    w, w_ld, N, w_scale, bias = _weight_of(weight, weight_scale, bias, K, x2.device)
-    with _on_device(x2.device) as stream:
-        out = torch.empty(lead + (N,), dtype=out_dtype, device=x2.device)
-        nbytes = lib.uhm_int8_matmul_workspace_bytes(M, N, K)
-        ws = _workspace(nbytes, x2.device)
-        _lib.check_model(lib.uhm_int8_matmul(x2.data_ptr(), x_ld, x_scale.data_ptr(), w.data_ptr(), w_ld, w_scale.data_ptr(), _ptr(bias),
-                                             out.data_ptr(), _UHM_DTYPES[out_dtype], M, N, K, _lib.UHM_RELU if relu else 0, _ptr(ws),
-                                             nbytes, stream), 'uhm_int8_matmul')
-    return out
+    return _lib.load_torch_ops().int8_matmul(x, x_scale, weight, weight_scale, bias, bool(relu), out_dtype)
 
 
 def int8_linear(x, weight, weight_scale, bias=None, relu=False):
     """A fully connected layer in 8-bit integers: the rows of x (float32 / bfloat16 / float16 [..., K]) are quantised on the way
     (quantize_rows) and multiplied with a weight that was quantised before (weight, weight_scale = quantize_rows(W), W [N, K])
     -> act(x . W^T + bias) [..., N] in x's type.  Evaluation only: no gradient."""
-    lib = _lib.load_model_ops()
-    x2, lead, K, dtype = _float_rows(x, 'x')
-    _no_grad_wanted([t for t in (x, weight_scale, bias) if isinstance(t, torch.Tensor)], 'int8_linear')
-    M = x2.shape[0]
-    w, w_ld, N, w_scale, bias = _weight_of(weight, weight_scale, bias, K, x2.device)
-    with _on_device(x2.device) as stream:
-        out = torch.empty(lead + (N,), dtype=x.dtype, device=x2.device)
-        nbytes = lib.uhm_int8_linear_workspace_bytes(M, N, K)
-        ws = _workspace(nbytes, x2.device)
-        _lib.check_model(lib.uhm_int8_linear(x2.data_ptr(), dtype, _ld(x2), w.data_ptr(), w_ld, w_scale.data_ptr(), _ptr(bias),
-                                             out.data_ptr(), M, N, K, _lib.UHM_RELU if relu else 0, _ptr(ws), nbytes, stream),
-                         'uhm_int8_linear')
-    return out
+    return _lib.load_torch_ops().int8_linear(x, weight, weight_scale, bias, bool(relu))
