@@ -313,8 +313,8 @@ __global__ __launch_bounds__(T) void quantize_rows_kernel(const void* __restrict
 // Up to MB tokens per block: bound by the one read of the weight.  A block of T threads owns R channels and all of K (no split, no
 // join, one launch): thread t holds bytes 16 t .. 16 t + 15 of every T * 16, AHEAD steps of every channel's row are in flight, products on
 // the 4-way dot instruction (for so few tokens they take less time than the loads).  X < 0: tokens in 8 bits.  X >= 0: ONE token
-// of that float type, quantised here: every block finds the row's maximum again (the row comes out of the L2) while its weight
-// loads are on their way, and rounds its chunks as it needs them.
+// of that float type, quantised here: every block finds the row's maximum again (the row comes out of the L2) and keeps its chunks
+// in registers until then (those past AHEAD steps are read again).
 template <int T, int R, int MB, int X>
 __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x, long long x_ld, int aligned, const int8_t* __restrict__ b,
                                                      long long b_ld, int M, int N, int K, const Epilogue e) {
@@ -326,6 +326,16 @@ __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x,
     const int8_t* pb[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) pb[r] = b + min(n0 + r, (long long)N - 1) * b_ld;
+    // a float token first: its maximum is found while the weight loads behind it are on their way (loads return in order)
+    constexpr int HELD = X >= 0 ? AHEAD : 0;
+    F4 held[HELD + 1][4];
+    if constexpr (X >= 0) {
+#pragma unroll
+        for (int p = 0; p < HELD; ++p)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) held[p][j] = load4<X>(x, min(p * STEP + tid * 16 + 4 * j, (K - 1) & ~3), K, aligned);
+        __builtin_amdgcn_sched_barrier(0);
+    }
     v4i w[AHEAD][R];
     auto fetch = [&](int p, int k) {
 #pragma unroll
@@ -337,14 +347,13 @@ __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x,
     RowScale s = {0.f, 0.f};
     const int8_t* px[MB];
     if constexpr (X >= 0) {
+        __builtin_amdgcn_sched_barrier(0);
         unsigned top = 0;
-        for (int k = tid * 4; k < K; k += 32 * T) {
-            F4 h[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[i] = load4<X>(x, min(k + i * T * 4, (K - 1) & ~3), K, aligned);
+        for (int p = 0; p < HELD; ++p)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, top_of(h[i]));
-        }
+            for (int j = 0; j < 4; ++j) top = max(top, top_of(held[p][j]));
+        for (int k = HELD * STEP + tid * 4; k < K; k += T * 4) top = max(top, top_of(load4<X>(x, k, K, aligned)));
         s = row_scale(block_max<T>(top));
     } else {
 #pragma unroll
@@ -356,28 +365,38 @@ __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x,
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int m = 0; m < MB; ++m) acc[r][m] = 0;
-    for (int base = 0; base < K; base += AHEAD * STEP) {
+    auto step = [&](int p, int k, const v4i (&xv)[MB]) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int m = 0; m < MB; ++m)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[r][m] = __builtin_amdgcn_sdot4(w[p][r][j], xv[m][j], acc[r][m], false);
+        if (k + AHEAD * STEP < K) fetch(p, k + AHEAD * STEP);          // (what it leaves stale meets zeros)
+    };
+    if constexpr (X >= 0) {
+#pragma unroll
+        for (int p = 0; p < HELD; ++p) {
+            const int k = p * STEP + tid * 16;
+            v4i xv[1];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) xv[0][j] = k + 4 * j < K ? (int)quantise4(held[p][j], s) : 0;
+            step(p, k, xv);
+        }
+    }
+    for (int base = HELD * STEP; base < K; base += AHEAD * STEP) {
 #pragma unroll
         for (int p = 0; p < AHEAD; ++p) {
             const int k = base + p * STEP + tid * 16;
             v4i xv[MB];
             if constexpr (X >= 0) {
-                xv[0] = v4i{0, 0, 0, 0};
-                if (k < K) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) xv[0][j] = (int)quantise4(load4<X>(x, k + 4 * j, K, aligned), s);
-                }
+                for (int j = 0; j < 4; ++j) xv[0][j] = k + 4 * j < K ? (int)quantise4(load4<X>(x, k + 4 * j, K, aligned), s) : 0;
             } else {
 #pragma unroll
                 for (int m = 0; m < MB; ++m) xv[m] = load16(px[m], k, K, true);
             }
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int m = 0; m < MB; ++m)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[r][m] = __builtin_amdgcn_sdot4(w[p][r][j], xv[m][j], acc[r][m], false);
-            if (k + AHEAD * STEP < K) fetch(p, k + AHEAD * STEP);      // (what it leaves stale meets zeros)
+            step(p, k, xv);
         }
     }
 
@@ -477,14 +496,14 @@ int launch_few(const void* x, long long x_ld, int al, const int8_t* b, long long
     auto launch = [&](auto kernel, int threads, int R) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)(((long long)N + R - 1) / R), (unsigned)((M + MB - 1) / MB)), dim3(threads), 0, s, x, x_ld, al, b, b_ld, M, N, K, e);
     };
-    // threads by K (two to four steps of 16 bytes each), channels per block by N: at least a block for every CU before a block takes more
+    // threads by K (up to four steps of 16 bytes each, then loops), channels per block by N: at least a block for every CU before a block takes more
     auto rows = [&](auto t) {
         constexpr int T = decltype(t)::value;
         if (N >= 1024) launch(int8_few_kernel<T, 4, MB, X>, T, 4);
         else if (N >= 512) launch(int8_few_kernel<T, 2, MB, X>, T, 2);
         else launch(int8_few_kernel<T, 1, MB, X>, T, 1);
     };
-    if (K <= 2048) rows(std::integral_constant<int, 64>{});
+    if (K <= 4096) rows(std::integral_constant<int, 64>{});
     else if (K <= 16384) rows(std::integral_constant<int, 256>{});
     else rows(std::integral_constant<int, 512>{});
     return (int)hipGetLastError();

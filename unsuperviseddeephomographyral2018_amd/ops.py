@@ -732,7 +732,8 @@ def global_norm(tensors):
 
 def clip_by_global_norm(tensors, clip_norm, use_norm=None):
     """tf.clip_by_global_norm: -> (list of t * clip_norm / max(norm, clip_norm), norm), in each tensor's type.  A norm that is not
-    finite makes every value NaN.  use_norm: a norm computed before (float32 scalar on the device).  No gradient."""
+    finite makes every value NaN.  use_norm: a norm computed before (float32 scalar on the device).  Small results share one
+    allocation (it lives as long as any of them).  No gradient."""
     return _lib.load_torch_ops().clip_by_global_norm(tensors, clip_norm, use_norm)
 
 
