@@ -43,19 +43,21 @@ __device__ __forceinline__ void put(void* out, int dtype, size_t at, float v) {
     else ((_Float16*)out)[at] = (_Float16)v;
 }
 
+// the first `keep` of 16 bytes, zeros behind them
+__device__ __forceinline__ v4i keep_first(v4i v, int keep) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int b = keep - 4 * j;                                    // bytes of word j that count
+        v[j] &= b >= 4 ? -1 : (b <= 0 ? 0 : (int)((1u << (8 * b)) - 1u));
+    }
+    return v;
+}
 // the 16 bytes of a row from k on, zero behind K (one operand's zeros are enough for the product, the other's bytes may be anything)
-__device__ __forceinline__ v4i load16(const int8_t* row, long long k, long long K, bool mask_tail) {
+__device__ __forceinline__ v4i load16(const int8_t* row, int k, int K, bool mask_tail) {
     v4i v = {0, 0, 0, 0};
     if (k < K) {
         v = *reinterpret_cast<const v4i*>(row + k);
-        if (mask_tail && K - k < 16) {
-            const int keep = (int)(K - k);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int b = keep - 4 * j;                            // bytes of word j that count
-                v[j] &= b >= 4 ? -1 : (b <= 0 ? 0 : (int)((1u << (8 * b)) - 1u));
-            }
-        }
+        if (mask_tail) v = keep_first(v, K - k);
     }
     return v;
 }
@@ -95,7 +97,8 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void int8_matmul_kernel(const int8
     // last one repeat it (their outputs are not written)
     const int8_t* const base_a = a + m0 * a_ld;
     const int8_t* const base_b = b + n0 * b_ld;
-    const unsigned chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+    static_assert(WAVES % 2 == 0, "the chunk order of a load depends on its wave alone");
+    const unsigned chunk = ((lane & 7) ^ ((wave & 1) * 4 + (lane >> 4))) * 16;
     unsigned row_a[LA], row_b[LB];                                        // (256 rows of at most MAX_LD: 32 bits)
 #pragma unroll
     for (int i = 0; i < LA; ++i) row_a[i] = (unsigned)min((long long)(i * WAVES + wave) * 8 + (lane >> 3), M - 1 - m0) * (unsigned)a_ld;
@@ -140,7 +143,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void int8_matmul_kernel(const int8
         // the operands of step s + 1 are read while the matrix instructions of step s run, and no earlier: two sets of registers
         v4i fa[2][TM], fb[2][TN];
         auto read = [&](int s) {
-            const int c = (2 * s + half) ^ (row & 7);
+            const int c = (2 * s + half) ^ (row >> 1 & 7);
 #pragma unroll
             for (int i = 0; i < TM; ++i) fa[s & 1][i] = sa[buf][(wm + i * 32 + row) * 8 + c];
 #pragma unroll
@@ -247,23 +250,34 @@ __device__ __forceinline__ float value(typename Raw<T>::type r) {
     else if constexpr (T == UHM_BF16) return __uint_as_float((unsigned)r << 16);
     else return __half2float(__ushort_as_half(r));
 }
-// elements k .. k + 3 of a row, zeros behind K (k % 4 == 0).  `aligned`: the row starts on four elements
-template <int T>
-__device__ __forceinline__ F4 load4(const void* row, int k, int K, bool aligned) {
-    using raw = typename Raw<T>::type;
+// Elements k .. k + 3 of a row (k % 4 == 0), zeros behind K.  WHOLE: rows start on four elements and K ends on four; a load has no
+// branch then (past K the last four are given again: they change no maximum, and the caller drops them), so that many are in flight.
+template <int X, bool WHOLE>
+__device__ __forceinline__ F4 load4(const void* row, int k, int K) {
+    using raw = typename Raw<X>::type;
     struct alignas(4 * sizeof(raw)) R4 { raw v[4]; };
-    const raw* p = (const raw*)row + k;
     F4 x = {{0.f, 0.f, 0.f, 0.f}};
-    if (aligned && k + 4 <= K) {
-        const R4 r = *reinterpret_cast<const R4*>(p);
+    if constexpr (WHOLE) {
+        const R4 r = *reinterpret_cast<const R4*>((const raw*)row + min(k, K - 4));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x.v[j] = value<T>(r.v[j]);
+        for (int j = 0; j < 4; ++j) x.v[j] = value<X>(r.v[j]);
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (k + j < K) x.v[j] = value<T>(p[j]);
+            if (k + j < K) x.v[j] = value<X>(((const raw*)row)[k + j]);
     }
     return x;
+}
+// COUNT of them, STEP elements apart
+template <int X, int COUNT>
+__device__ __forceinline__ void load4s(F4 (&x)[COUNT], const void* row, int k, int step, int K, int whole) {
+    if (whole) {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) x[i] = load4<X, true>(row, k + i * step, K);
+    } else {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) x[i] = load4<X, false>(row, k + i * step, K);
+    }
 }
 
 // the largest of `top` over a block of T threads, in every thread
@@ -285,38 +299,42 @@ __device__ __forceinline__ unsigned block_max(unsigned top) {
 // a longer one is read a second time (out of the L2).  All of a thread's loads are in flight together.
 template <int X, int T>
 __global__ __launch_bounds__(T) void quantize_rows_kernel(const void* __restrict__ x, long long x_ld, int8_t* __restrict__ q,
-                                                          long long q_ld, float* __restrict__ scale, int K, int aligned) {
-    constexpr int HELD = 8;
+                                                          long long q_ld, float* __restrict__ scale, int K, int whole) {
+    constexpr int HELD = 8, SEGMENT = HELD * T * 4;
     const size_t row = blockIdx.x;
     const char* px = (const char*)x + row * x_ld * sizeof(typename Raw<X>::type);
-    const int padded = (K + 15) & ~15;
+    const int padded = (K + 15) & ~15, k0 = threadIdx.x * 4;
     F4 held[HELD];
     unsigned top = 0;
+    for (int base = SEGMENT; base < K; base += SEGMENT) {
+        load4s<X>(held, px, base + k0, T * 4, K, whole);
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) held[i] = load4<X>(px, min(threadIdx.x + i * T, (unsigned)(padded - 1) / 4) * 4, K, aligned);
+        for (int i = 0; i < HELD; ++i) top = max(top, top_of(held[i]));
+    }
+    load4s<X>(held, px, k0, T * 4, K, whole);
 #pragma unroll
     for (int i = 0; i < HELD; ++i) top = max(top, top_of(held[i]));
-    for (int k = (HELD * T + threadIdx.x) * 4; k < K; k += T * 4) top = max(top, top_of(load4<X>(px, k, K, aligned)));
     const RowScale s = row_scale(block_max<T>(top));
     if (threadIdx.x == 0) scale[row] = s.scale;
     int8_t* pq = q + row * q_ld;
+    for (int base = 0; base < padded; base += SEGMENT) {
+        if (base) load4s<X>(held, px, base + k0, T * 4, K, whole);
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        const int k = (threadIdx.x + i * T) * 4;
-        if (k < padded) *reinterpret_cast<unsigned*>(pq + k) = quantise4(held[i], s);
+        for (int i = 0; i < HELD; ++i) {
+            const int k = base + k0 + i * T * 4;
+            if (k < padded) *reinterpret_cast<unsigned*>(pq + k) = k < K ? quantise4(held[i], s) : 0;
+        }
     }
-    for (int k = (HELD * T + threadIdx.x) * 4; k < padded; k += T * 4)
-        *reinterpret_cast<unsigned*>(pq + k) = quantise4(load4<X>(px, k, K, aligned), s);
 }
 
 // ---- few tokens -----------------------------------------------------------------------------------------------------------------
 // Up to MB tokens per block: bound by the one read of the weight.  A block of T threads owns R channels and all of K (no split, no
 // join, one launch): thread t holds bytes 16 t .. 16 t + 15 of every T * 16, AHEAD steps of every channel's row are in flight, products on
 // the 4-way dot instruction (for so few tokens they take less time than the loads).  X < 0: tokens in 8 bits.  X >= 0: ONE token
-// of that float type, quantised here: every block finds the row's maximum again (the row comes out of the L2) and keeps its chunks
-// in registers until then (those past AHEAD steps are read again).
+// of that float type, quantised here: every block finds the row's maximum again (the row comes out of the L2) and keeps AHEAD
+// steps of it in registers until then (what is longer is read again).
 template <int T, int R, int MB, int X>
-__global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x, long long x_ld, int aligned, const int8_t* __restrict__ b,
+__global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x, long long x_ld, int whole, const int8_t* __restrict__ b,
                                                      long long b_ld, int M, int N, int K, const Epilogue e) {
     static_assert(X < 0 || MB == 1, "one token");
     constexpr int STEP = T * 16, AHEAD = R * MB >= 16 ? 2 : 4;
@@ -326,20 +344,22 @@ __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x,
     const int8_t* pb[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) pb[r] = b + min(n0 + r, (long long)N - 1) * b_ld;
-    // a float token first: its maximum is found while the weight loads behind it are on their way (loads return in order)
-    constexpr int HELD = X >= 0 ? AHEAD : 0;
-    F4 held[HELD + 1][4];
+    // a float token first: its maximum is found while the weight loads behind it are on their way (loads return in order).  Thread t
+    // holds elements 4 t .. 4 t + 3 of every T * 4 -- consecutive lanes, consecutive memory: 16 elements a lane as the dot products
+    // want them would take four times as many cycles per load (fc1: 5 us more) -- and hands them over in LDS, in 8 bits.
+    constexpr int SEGMENT = AHEAD * STEP, HELD = X >= 0 ? SEGMENT / (T * 4) : 1;
+    __shared__ v4i row8[X >= 0 ? SEGMENT / 16 : 1];
+    F4 held[HELD];
     if constexpr (X >= 0) {
-#pragma unroll
-        for (int p = 0; p < HELD; ++p)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) held[p][j] = load4<X>(x, min(p * STEP + tid * 16 + 4 * j, (K - 1) & ~3), K, aligned);
+        load4s<X>(held, x, tid * 4, T * 4, K, whole);
         __builtin_amdgcn_sched_barrier(0);
     }
+    // loads without a branch: past K the last 16 bytes again, which meet zeros of the token
+    const int last = (K - 1) & ~15;
     v4i w[AHEAD][R];
     auto fetch = [&](int p, int k) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) w[p][r] = load16(pb[r], k, K, false);
+        for (int r = 0; r < R; ++r) w[p][r] = *reinterpret_cast<const v4i*>(pb[r] + min(k, last));
     };
 #pragma unroll
     for (int p = 0; p < AHEAD; ++p) fetch(p, p * STEP + tid * 16);
@@ -350,10 +370,13 @@ __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x,
         __builtin_amdgcn_sched_barrier(0);
         unsigned top = 0;
 #pragma unroll
-        for (int p = 0; p < HELD; ++p)
+        for (int i = 0; i < HELD; ++i) top = max(top, top_of(held[i]));
+        for (int base = SEGMENT; base < K; base += SEGMENT) {
+            F4 more[HELD];
+            load4s<X>(more, x, base + tid * 4, T * 4, K, whole);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) top = max(top, top_of(held[p][j]));
-        for (int k = HELD * STEP + tid * 4; k < K; k += T * 4) top = max(top, top_of(load4<X>(x, k, K, aligned)));
+            for (int i = 0; i < HELD; ++i) top = max(top, top_of(more[i]));
+        }
         s = row_scale(block_max<T>(top));
     } else {
 #pragma unroll
@@ -372,29 +395,34 @@ __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x,
             for (int m = 0; m < MB; ++m)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[r][m] = __builtin_amdgcn_sdot4(w[p][r][j], xv[m][j], acc[r][m], false);
-        if (k + AHEAD * STEP < K) fetch(p, k + AHEAD * STEP);          // (what it leaves stale meets zeros)
+        if (k - tid * 16 + SEGMENT < K) fetch(p, k + SEGMENT);
     };
-    if constexpr (X >= 0) {
+    for (int base = 0; base < K; base += SEGMENT) {
+        if constexpr (X >= 0) {
+            if (base) {
+                load4s<X>(held, x, base + tid * 4, T * 4, K, whole);      // (again, out of the L2)
+                __syncthreads();                                   // everyone is through with the segment before
+            }
 #pragma unroll
-        for (int p = 0; p < HELD; ++p) {
-            const int k = p * STEP + tid * 16;
-            v4i xv[1];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) xv[0][j] = k + 4 * j < K ? (int)quantise4(held[p][j], s) : 0;
-            step(p, k, xv);
+            for (int i = 0; i < HELD; ++i) {
+                const int k = base + (i * T + tid) * 4;
+                reinterpret_cast<unsigned*>(row8)[i * T + tid] = k < K ? quantise4(held[i], s) : 0;
+            }
+            __syncthreads();
         }
-    }
-    for (int base = HELD * STEP; base < K; base += AHEAD * STEP) {
 #pragma unroll
         for (int p = 0; p < AHEAD; ++p) {
             const int k = base + p * STEP + tid * 16;
             v4i xv[MB];
             if constexpr (X >= 0) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) xv[0][j] = k + 4 * j < K ? (int)quantise4(load4<X>(x, k + 4 * j, K, aligned), s) : 0;
+                xv[0] = row8[p * T + tid];
             } else {
 #pragma unroll
-                for (int m = 0; m < MB; ++m) xv[m] = load16(px[m], k, K, true);
+                for (int m = 0; m < MB; ++m) xv[m] = *reinterpret_cast<const v4i*>(px[m] + min(k, last));
+                if (base + (p + 1) * STEP > K) {                   // (the same for every thread)
+#pragma unroll
+                    for (int m = 0; m < MB; ++m) xv[m] = keep_first(xv[m], K - k);
+                }
             }
             step(p, k, xv);
         }
@@ -427,7 +455,7 @@ __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x,
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 constexpr long long MAX_K = 131071, MAX_DIM = 0x7fffffffLL - 512;
 constexpr long long MAX_LD = 1LL << 23;     // 256 rows of it are indexed in 32 bits
-constexpr long long FEW = 4;               // tokens up to which the weight is read by int8_few_kernel
+constexpr long long FEW = 2;               // tokens up to which int8_few_kernel reads the weight (fc1: 2 tokens 10.7 us, 4 12.5; tiles, 8 tokens, 12.2)
 
 struct Plan { int bm, bn, splits, tiles_per_split; };
 
@@ -472,15 +500,15 @@ int check_operands(const void* x, long long x_ld, const int8_t* b, long long b_l
     return 0;
 }
 
-// the row starts on four elements
-inline int rows_aligned(const void* x, int dtype, long long x_ld, long long rows) {
+// rows start and end on four elements
+inline int rows_whole(const void* x, int dtype, long long x_ld, long long rows, long long K) {
     const uintptr_t size = dtype == UHM_F32 ? 4 : 2;
-    return (((uintptr_t)x | (rows > 1 ? (uintptr_t)x_ld * size : 0)) & (4 * size - 1)) == 0;
+    return K % 4 == 0 && (((uintptr_t)x | (rows > 1 ? (uintptr_t)x_ld * size : 0)) & (4 * size - 1)) == 0;
 }
 
 template <int X>
 int quantize_rows(const void* x, long long x_ld, int8_t* q, long long q_ld, float* scale, long long rows, long long K, hipStream_t s) {
-    const int al = rows_aligned(x, X, x_ld, rows);
+    const int al = rows_whole(x, X, x_ld, rows, K);
     // as few threads as hold the row in registers
     auto launch = [&](auto kernel, int threads) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(threads), 0, s, x, x_ld, q, q_ld, scale, (int)K, al);
@@ -512,8 +540,7 @@ int launch_few(const void* x, long long x_ld, int al, const int8_t* b, long long
 int product(const int8_t* a, long long a_ld, const int8_t* b, long long b_ld, long long M, long long N, long long K, const Epilogue& e, int* sums,
             hipStream_t s) {
     if (M <= 1) return launch_few<1, -1>(a, a_ld, 1, b, b_ld, (int)M, (int)N, (int)K, e, s);
-    if (M <= 2) return launch_few<2, -1>(a, a_ld, 1, b, b_ld, (int)M, (int)N, (int)K, e, s);
-    if (M <= FEW) return launch_few<4, -1>(a, a_ld, 1, b, b_ld, (int)M, (int)N, (int)K, e, s);
+    if (M <= FEW) return launch_few<2, -1>(a, a_ld, 1, b, b_ld, (int)M, (int)N, (int)K, e, s);
     const Plan p = plan_of(M, N, K);
     const int mt = (int)((M + p.bm - 1) / p.bm), nt = (int)((N + p.bn - 1) / p.bn);
     if (p.splits == 1) sums = nullptr;
@@ -564,7 +591,7 @@ using namespace uhm;
 extern "C" int uhm_quantize_rows(const void* x, int dtype, long long x_ld, int8_t* q, long long q_ld, float* scale, long long rows,
                                  long long K, uhm_stream_t stream) {
     if (rows < 0 || K < 1 || x_ld < K || q_ld < K) return UHM_E_SHAPE;
-    if (rows > MAX_DIM || K > MAX_DIM - 8192) return UHM_E_TOO_LARGE;      // (a thread's index goes one step past K)
+    if (rows > MAX_DIM || K > MAX_DIM - 65536) return UHM_E_TOO_LARGE;      // (indexes go one segment past K)
     if (dtype < UHM_F32 || dtype > UHM_F16) return UHM_E_DTYPE;
     if (rows == 0) return 0;
     if (!x || !q || !scale) return UHM_E_NULL;
@@ -607,7 +634,7 @@ extern "C" int uhm_int8_linear(const void* x, int dtype, long long x_ld, const i
     hipStream_t s = (hipStream_t)stream;
     Epilogue e = {nullptr, b_scale, bias, out, dtype, (flags & UHM_RELU) ? 1 : 0};
     if (M == 1) {
-        const int al = rows_aligned(x, dtype, x_ld, 1);
+        const int al = rows_whole(x, dtype, x_ld, 1, K);
         if (dtype == UHM_F32) return launch_few<1, UHM_F32>(x, x_ld, al, b, b_ld, 1, (int)N, (int)K, e, s);
         if (dtype == UHM_BF16) return launch_few<1, UHM_BF16>(x, x_ld, al, b, b_ld, 1, (int)N, (int)K, e, s);
         return launch_few<1, UHM_F16>(x, x_ld, al, b, b_ld, 1, (int)N, (int)K, e, s);
