@@ -21,8 +21,6 @@ namespace uhm {
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 
-constexpr int BK = 128;                    // bytes of K per tile
-
 struct Epilogue {
     const float* a_scale;
     const float* b_scale;
@@ -79,31 +77,34 @@ template <int N> __device__ __forceinline__ void wait_for_loads() {          // 
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
 }
 
-template <int BM, int BN, int WM, int WN, int STAGES>      // WM x WN waves, each (BM / WM) x (BN / WN) outputs
+template <int BM, int BN, int BK, int WM, int WN, int STAGES>      // WM x WN waves, each (BM / WM) x (BN / WN) outputs
 __global__ __launch_bounds__(WM * WN * 64, 1) void int8_matmul_kernel(const int8_t* __restrict__ a, long long a_ld, const int8_t* __restrict__ b,
                                                                       long long b_ld, int M, int N, int K, int mt, int nt, int splits,
                                                                       int tiles_per_split, int* __restrict__ sums, const Epilogue e) {
     constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
-    constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;           // loads (8 rows of 128 bytes each) of a wave per tile
-    static_assert(LA >= 1 && LB >= 1 && LA * WAVES * 8 == BM && LB * WAVES * 8 == BN, "staging");
-    __shared__ v4i sa[STAGES][BM * 8], sb[STAGES][BN * 8];
+    // a tile's row is C chunks of 16 bytes; chunk c of row r sits at c ^ (r / PERIOD % C): 16 lanes that read one chunk of 16 rows at once
+    // meet all 64 banks
+    constexpr int C = BK / 16, PERIOD = 256 / BK, RL = 64 / C;         // RL: rows of one load of a wave
+    constexpr int LA = BM / RL / WAVES, LB = BN / RL / WAVES;         // loads of a wave per tile
+    static_assert(LA >= 1 && LB >= 1 && LA * WAVES * RL == BM && LB * WAVES * RL == BN, "staging");
+    static_assert((WAVES * RL) % 16 == 0, "the chunk order of a load depends on its wave alone");
+    __shared__ v4i sa[STAGES][BM * C], sb[STAGES][BN * C];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
     const Place at = place(mt, nt, splits);
     const long long m0 = (long long)at.m * BM, n0 = (long long)at.n * BN;
     const int t0 = at.z * tiles_per_split, t1 = min(t0 + tiles_per_split, (K + BK - 1) / BK), whole = min(t1, K / BK);
 
-    // this lane's 16 bytes of each load: row lane / 8 of eight, the chunk that belongs at position lane % 8 of it; rows behind the
-    // last one repeat it (their outputs are not written)
+    // this lane's 16 bytes of each load: row lane / C, the chunk that belongs at position lane % C of it; rows behind the last one
+    // repeat it (their outputs are not written)
     const int8_t* const base_a = a + m0 * a_ld;
     const int8_t* const base_b = b + n0 * b_ld;
-    static_assert(WAVES % 2 == 0, "the chunk order of a load depends on its wave alone");
-    const unsigned chunk = ((lane & 7) ^ ((wave & 1) * 4 + (lane >> 4))) * 16;
+    const unsigned chunk = ((lane % C) ^ ((wave * RL + lane / C) / PERIOD % C)) * 16;
     unsigned row_a[LA], row_b[LB];                                        // (256 rows of at most MAX_LD: 32 bits)
 #pragma unroll
-    for (int i = 0; i < LA; ++i) row_a[i] = (unsigned)min((long long)(i * WAVES + wave) * 8 + (lane >> 3), M - 1 - m0) * (unsigned)a_ld;
+    for (int i = 0; i < LA; ++i) row_a[i] = (unsigned)min((long long)(i * WAVES + wave) * RL + lane / C, M - 1 - m0) * (unsigned)a_ld;
 #pragma unroll
-    for (int i = 0; i < LB; ++i) row_b[i] = (unsigned)min((long long)(i * WAVES + wave) * 8 + (lane >> 3), N - 1 - n0) * (unsigned)b_ld;
+    for (int i = 0; i < LB; ++i) row_b[i] = (unsigned)min((long long)(i * WAVES + wave) * RL + lane / C, N - 1 - n0) * (unsigned)b_ld;
     auto to_lds = [](const int8_t* p, v4i* s) {
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)s, 16, 0, 0);
     };
@@ -143,11 +144,11 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void int8_matmul_kernel(const int8
         // the operands of step s + 1 are read while the matrix instructions of step s run, and no earlier: two sets of registers
         v4i fa[2][TM], fb[2][TN];
         auto read = [&](int s) {
-            const int c = (2 * s + half) ^ (row >> 1 & 7);
+            const int c = (2 * s + half) ^ (row / PERIOD % C);
 #pragma unroll
-            for (int i = 0; i < TM; ++i) fa[s & 1][i] = sa[buf][(wm + i * 32 + row) * 8 + c];
+            for (int i = 0; i < TM; ++i) fa[s & 1][i] = sa[buf][(wm + i * 32 + row) * C + c];
 #pragma unroll
-            for (int j = 0; j < TN; ++j) fb[s & 1][j] = sb[buf][(wn + j * 32 + row) * 8 + c];
+            for (int j = 0; j < TN; ++j) fb[s & 1][j] = sb[buf][(wn + j * 32 + row) * C + c];
         };
         read(0);
 #pragma unroll
@@ -162,6 +163,13 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void int8_matmul_kernel(const int8
         buf = buf + 1 == STAGES ? 0 : buf + 1;
     }
 
+    // the tokens' scales through LDS: a load from memory for every row, one after the other, took 15 us of 4096 x 4096 outputs
+    float* const scales = reinterpret_cast<float*>(&sa[0][0]);
+    if (!sums) {
+        __syncthreads();
+        for (int i = tid; i < BM; i += WAVES * 64) scales[i] = e.a_scale[min(m0 + i, (long long)M - 1)];
+        __syncthreads();
+    }
     // D of a 32 x 32 tile: lane l, register i hold row 8 (i / 4) + 4 (l / 32) + i % 4, column l % 32
     auto each = [&](auto out) {
         float sbn[TN], bias[TN];
@@ -171,30 +179,33 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void int8_matmul_kernel(const int8
             sbn[j] = sums ? 0.f : e.b_scale[n];
             bias[j] = sums || !e.bias ? 0.f : e.bias[n];
         }
-        int m = (int)m0 + wm + half * 4;
-        size_t at = (size_t)m * N + n0 + wn + row;
+        int m = wm + half * 4;
+        size_t at = (size_t)(m0 + m) * N + n0 + wn + row;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                asm volatile("" : "+v"(m), "+v"(at));            // (one row's address at a time: all of them at once would spill)
-                if (m < M) {
+            for (int q = 0; q < 4; ++q) {
+                asm volatile("" : "+v"(m), "+v"(at));            // (a few rows' addresses at a time: all of them at once would spill)
+                const float4 s4 = sums ? float4{} : *reinterpret_cast<const float4*>(scales + m);
+                const float sam[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-                    for (int j = 0; j < TN; ++j)
-                        if (n0 + wn + j * 32 + row < N) out(at + j * 32, acc[i][j][k], m, sbn[j], bias[j]);
-                }
-                const int step = (k & 3) == 3 ? 5 : 1;
-                m += step;
-                at += step * (size_t)N;
+                for (int k = 0; k < 4; ++k)
+                    if (m0 + m + k < M) {
+#pragma unroll
+                        for (int j = 0; j < TN; ++j)
+                            if (n0 + wn + j * 32 + row < N) out(at + k * (size_t)N + j * 32, acc[i][j][4 * q + k], sam[k], sbn[j], bias[j]);
+                    }
+                m += 8;
+                at += 8 * (size_t)N;
             }
     };
     if (sums) {
         int* part = sums + (size_t)at.z * M * N;
-        each([&](size_t at, int v, int, float, float) { part[at] = v; });
+        each([&](size_t at, int v, float, float, float) { part[at] = v; });
     } else if (e.dtype == UHM_F32) {
-        each([&](size_t at, int v, int m, float sbn, float bias) { ((float*)e.out)[at] = finish(v, e.a_scale[m], sbn, bias, e.relu); });
+        each([&](size_t at, int v, float sam, float sbn, float bias) { ((float*)e.out)[at] = finish(v, sam, sbn, bias, e.relu); });
     } else {
-        each([&](size_t at, int v, int m, float sbn, float bias) { put(e.out, e.dtype, at, finish(v, e.a_scale[m], sbn, bias, e.relu)); });
+        each([&](size_t at, int v, float sam, float sbn, float bias) { put(e.out, e.dtype, at, finish(v, sam, sbn, bias, e.relu)); });
     }
 }
 
@@ -457,17 +468,18 @@ constexpr long long MAX_K = 131071, MAX_DIM = 0x7fffffffLL - 512;
 constexpr long long MAX_LD = 1LL << 23;     // 256 rows of it are indexed in 32 bits
 constexpr long long FEW = 2;               // tokens up to which int8_few_kernel reads the weight (fc1: 2 tokens 10.7 us, 4 12.5; tiles, 8 tokens, 12.2)
 
-struct Plan { int bm, bn, splits, tiles_per_split; };
+struct Plan { int bm, bn, bk, splits, tiles_per_split; };
 
 inline Plan plan_of(long long M, long long N, long long K) {
     const auto tiles_of = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
     Plan p;
+    p.bk = 128;
     long long most;                            // splits: past these the partial sums cost more than the blocks they add bring
     if (M <= 32) { p.bm = 32; p.bn = 128; most = 32; }
-    else if (tiles_of(256, 256) >= 200) { p.bm = p.bn = 256; most = 1; }
+    else if (tiles_of(256, 256) >= 200) { p.bm = p.bn = 256; p.bk = 64; most = 1; }
     else if (tiles_of(128, 128) >= 200) { p.bm = p.bn = 128; most = 1; }
     else { p.bm = p.bn = 64; most = 16; }
-    const long long tiles = tiles_of(p.bm, p.bn), kt = (K + BK - 1) / BK;
+    const long long tiles = tiles_of(p.bm, p.bn), kt = (K + p.bk - 1) / p.bk;
     long long s = tiles < 256 ? 512 / tiles : 1;
     if (s > most) s = most;
     if (s > kt / 8) s = kt / 8;                // at least 8 tiles of K each: a block's first loads take as long as several tiles
@@ -548,10 +560,10 @@ int product(const int8_t* a, long long a_ld, const int8_t* b, long long b_ld, lo
         hipLaunchKernelGGL(kernel, dim3((unsigned)mt * nt * p.splits), dim3(threads), 0, s, a, a_ld, b, b_ld, (int)M, (int)N, (int)K, mt, nt, p.splits,
                            p.tiles_per_split, sums, e);
     };
-    if (p.bm == 32) launch(int8_matmul_kernel<32, 128, 1, 4, 4>, 256);
-    else if (p.bm == 64) launch(int8_matmul_kernel<64, 64, 2, 2, 5>, 256);
-    else if (p.bm == 128) launch(int8_matmul_kernel<128, 128, 2, 2, 4>, 256);
-    else launch(int8_matmul_kernel<256, 256, 2, 4, 2>, 512);
+    if (p.bm == 32) launch(int8_matmul_kernel<32, 128, 128, 1, 4, 4>, 256);
+    else if (p.bm == 64) launch(int8_matmul_kernel<64, 64, 128, 2, 2, 5>, 256);
+    else if (p.bm == 128) launch(int8_matmul_kernel<128, 128, 128, 2, 2, 4>, 256);
+    else launch(int8_matmul_kernel<256, 256, 64, 2, 4, 5>, 512);
     if (int err = (int)hipGetLastError()) return err;
     if (p.splits > 1) {
         const long long blocks = (M * N + 255) / 256;
