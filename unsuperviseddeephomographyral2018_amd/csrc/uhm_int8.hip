@@ -3,13 +3,17 @@
 //   quantise:  top = max |x_r|, scale_r = top / 127, q = rne(x * (127 / top))
 //   product :  out[m, n] = act(sum_k a[m, k] b[n, k] * sa[m] * sb[n] + bias[n])        exact 32-bit integer sums
 //
-// Up to FEW tokens: int8_few_kernel, which streams the weight once.  More: one tiled kernel on v_mfma_i32_32x32x32_i8.  A block computes BM x BN outputs over a range of K: tiles of
-// BK = 128 bytes of BM rows of a and BN rows of b go global -> registers -> LDS (two buffers; the next tile's loads are in flight
-// while the present one is multiplied, one barrier per tile).  A tile row is 128 bytes = 8 chunks of 16; chunk c of row r sits at
-// position c ^ (r & 7), so that the 8 rows that 8 lanes read at once (one chunk each) cover all 64 banks' 128 bytes, and so does
-// a row that 8 lanes write.
-// Few rows leave few tiles (fc1 at 64 pairs: 8 of 64 x 128): the K range is split over gridDim.z blocks, each writes its 32-bit
-// sums to the workspace, and a second kernel adds them (integers: the split does not change the result) and applies the epilogue.
+// Up to FEW tokens: int8_few_kernel, which streams the weight once.  More: int8_matmul_kernel on v_mfma_i32_32x32x32_i8.  A block
+// computes BM x BN outputs over a range of K.  Tiles of BK = 128 bytes of BM rows of a and BN rows of b go from memory straight
+// into a ring of STAGES buffers in LDS; while one is multiplied the others are in flight (with 64 x 64 tiles two blocks of five
+// buffers fill a CU's 160 KB: the loads of fc1 outrun the latency of HBM), with one barrier per tile.
+// Few rows leave few tiles (fc1 at 64 pairs: 16 of 64 x 64): the K range is split over blocks, each writes its 32-bit sums to the
+// workspace, and int8_join_kernel adds them (integers: the split does not change the result) and applies the epilogue.
+//
+// Measured on one MI355X (launches of three sets of operands in turn, so that the weight comes from memory):
+//   fc1, 1024 x 32768:  1 pair 9.7 us (3.5 TB/s), from float 11.1; 64 pairs 13.0; 128 pairs from float 22 (quantising 6, product 11, join 4)
+//   4096 x 4096 x 8192: 147 us; each 8192 of K more take 115 us = 2.4 POP/s.  Its loop without loads takes 90 us, with neither loads
+//   nor LDS reads 69 us (the matrix instructions alone, at the clock that their power leaves): no latency is left to hide.
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -20,6 +24,8 @@ namespace uhm {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
+
+constexpr int BK = 128;                    // bytes of K per tile
 
 struct Epilogue {
     const float* a_scale;
@@ -77,7 +83,7 @@ template <int N> __device__ __forceinline__ void wait_for_loads() {          // 
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
 }
 
-template <int BM, int BN, int BK, int WM, int WN, int STAGES>      // WM x WN waves, each (BM / WM) x (BN / WN) outputs
+template <int BM, int BN, int WM, int WN, int STAGES>      // WM x WN waves, each (BM / WM) x (BN / WN) outputs
 __global__ __launch_bounds__(WM * WN * 64, 1) void int8_matmul_kernel(const int8_t* __restrict__ a, long long a_ld, const int8_t* __restrict__ b,
                                                                       long long b_ld, int M, int N, int K, int mt, int nt, int splits,
                                                                       int tiles_per_split, int* __restrict__ sums, const Epilogue e) {
@@ -129,38 +135,51 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void int8_matmul_kernel(const int8
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = v16i{};
 
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i)
-        if (t0 + i < t1) fetch(t0 + i, i);
+    // The operands of a step are read before the matrix instructions of the step before it run, also across tiles: the last step of
+    // a tile covers the barrier after which the next one may be read.  Behind it the tile's buffer is free and is filled again.
+    constexpr int STEPS = BK / 32;
+    static_assert(STEPS % 2 == 0, "two sets of operands");
     const int row = lane & 31, half = lane >> 5;
+    v4i fa[2][TM], fb[2][TN];
+    auto read = [&](int buf, int s) {
+        const int c = (2 * s + half) ^ (row / PERIOD % C);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) fa[s & 1][i] = sa[buf][(wm + i * 32 + row) * C + c];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) fb[s & 1][j] = sb[buf][(wn + j * 32 + row) * C + c];
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i)
+        if (t0 + i < t1) fetch(t0 + i, i);
+    if (t0 + STAGES - 1 < whole) wait_for_loads<(LA + LB) * (STAGES - 1)>();
+    else wait_for_loads<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
     int buf = 0;
+    if (t0 < t1) read(0, 0);
     for (int t = t0; t < t1; ++t) {
-        // tile t is in LDS for every wave, and none still reads the buffer that is filled next
-        if (t + STAGES - 2 < whole) wait_for_loads<(LA + LB) * (STAGES - 2)>();
-        else wait_for_loads<0>();
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (t + STAGES - 1 < t1) fetch(t + STAGES - 1, buf == 0 ? STAGES - 1 : buf - 1);
-        // the operands of step s + 1 are read while the matrix instructions of step s run, and no earlier: two sets of registers
-        v4i fa[2][TM], fb[2][TN];
-        auto read = [&](int s) {
-            const int c = (2 * s + half) ^ (row / PERIOD % C);
 #pragma unroll
-            for (int i = 0; i < TM; ++i) fa[s & 1][i] = sa[buf][(wm + i * 32 + row) * C + c];
-#pragma unroll
-            for (int j = 0; j < TN; ++j) fb[s & 1][j] = sb[buf][(wn + j * 32 + row) * C + c];
-        };
-        read(0);
-#pragma unroll
-        for (int s = 0; s < BK / 32; ++s) {
-            if (s + 1 < BK / 32) read(s + 1);
+        for (int s = 0; s < STEPS; ++s) {
+            if (s + 1 < STEPS) {
+                read(buf, s + 1);
+            } else if (t + 1 < t1) {
+                // tile t + 1 is in LDS for every wave, and none still reads tile t
+                if (t + STAGES - 1 < whole) wait_for_loads<(LA + LB) * (STAGES - 2)>();
+                else wait_for_loads<0>();
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                const int next = buf + 1 == STAGES ? 0 : buf + 1;
+                read(next, 0);
+                if (t + STAGES < t1) fetch(t + STAGES, buf);
+                buf = next;
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
                 for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[s & 1][i], fb[s & 1][j], acc[i][j], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
-        buf = buf + 1 == STAGES ? 0 : buf + 1;
     }
 
     // the tokens' scales through LDS: a load from memory for every row, one after the other, took 15 us of 4096 x 4096 outputs
@@ -468,18 +487,17 @@ constexpr long long MAX_K = 131071, MAX_DIM = 0x7fffffffLL - 512;
 constexpr long long MAX_LD = 1LL << 23;     // 256 rows of it are indexed in 32 bits
 constexpr long long FEW = 2;               // tokens up to which int8_few_kernel reads the weight (fc1: 2 tokens 10.7 us, 4 12.5; tiles, 8 tokens, 12.2)
 
-struct Plan { int bm, bn, bk, splits, tiles_per_split; };
+struct Plan { int bm, bn, splits, tiles_per_split; };
 
 inline Plan plan_of(long long M, long long N, long long K) {
     const auto tiles_of = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
     Plan p;
-    p.bk = 128;
     long long most;                            // splits: past these the partial sums cost more than the blocks they add bring
     if (M <= 32) { p.bm = 32; p.bn = 128; most = 32; }
-    else if (tiles_of(256, 256) >= 200) { p.bm = p.bn = 256; p.bk = 64; most = 1; }
+    else if (tiles_of(256, 256) >= 200) { p.bm = p.bn = 256; most = 1; }
     else if (tiles_of(128, 128) >= 200) { p.bm = p.bn = 128; most = 1; }
     else { p.bm = p.bn = 64; most = 16; }
-    const long long tiles = tiles_of(p.bm, p.bn), kt = (K + p.bk - 1) / p.bk;
+    const long long tiles = tiles_of(p.bm, p.bn), kt = (K + BK - 1) / BK;
     long long s = tiles < 256 ? 512 / tiles : 1;
     if (s > most) s = most;
     if (s > kt / 8) s = kt / 8;                // at least 8 tiles of K each: a block's first loads take as long as several tiles
@@ -560,10 +578,10 @@ int product(const int8_t* a, long long a_ld, const int8_t* b, long long b_ld, lo
         hipLaunchKernelGGL(kernel, dim3((unsigned)mt * nt * p.splits), dim3(threads), 0, s, a, a_ld, b, b_ld, (int)M, (int)N, (int)K, mt, nt, p.splits,
                            p.tiles_per_split, sums, e);
     };
-    if (p.bm == 32) launch(int8_matmul_kernel<32, 128, 128, 1, 4, 4>, 256);
-    else if (p.bm == 64) launch(int8_matmul_kernel<64, 64, 128, 2, 2, 5>, 256);
-    else if (p.bm == 128) launch(int8_matmul_kernel<128, 128, 128, 2, 2, 4>, 256);
-    else launch(int8_matmul_kernel<256, 256, 64, 2, 4, 5>, 512);
+    if (p.bm == 32) launch(int8_matmul_kernel<32, 128, 1, 4, 4>, 256);
+    else if (p.bm == 64) launch(int8_matmul_kernel<64, 64, 2, 2, 5>, 256);
+    else if (p.bm == 128) launch(int8_matmul_kernel<128, 128, 2, 2, 4>, 256);
+    else launch(int8_matmul_kernel<256, 256, 2, 4, 2>, 512);
     if (int err = (int)hipGetLastError()) return err;
     if (p.splits > 1) {
         const long long blocks = (M * N + 255) / 256;
