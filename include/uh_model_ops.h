@@ -67,7 +67,8 @@ UHM_API int uhm_global_norm(const void* const* tensors, const long long* numel, 
 /* out[i] = tensors[i] * f,  f = clip_norm / n if n > clip_norm, else 1; NaN if n is not finite (as tf.clip_by_global_norm: every
  * value becomes NaN).  n = use_norm[0] when use_norm (a device scalar) is given, else the global norm; norm[0] <- n (norm may
  * be NULL).  out[i] may equal tensors[i] (in place; with f = 1 nothing is then written); any other overlap of an output is
- * UHM_E_OVERLAP.  0 < clip_norm (may be +inf).  Workspace may be NULL when use_norm is given.                                */
+ * UHM_E_OVERLAP, of norm and use_norm too (they may be the same).  0 < clip_norm (may be +inf).  Workspace may be NULL when use_norm
+ * is given.                                */
 UHM_API int uhm_clip_by_global_norm(const void* const* tensors, void* const* out, const long long* numel, const int* dtypes,
                                     int count, float clip_norm, const float* use_norm, float* norm, void* workspace,
                                     size_t workspace_bytes, uhm_stream_t stream);
@@ -96,7 +97,8 @@ UHM_API int uhm_quantize_rows(const void* x, int dtype, long long x_ld, int8_t* 
                               long long K, uhm_stream_t stream);
 
 /* out [M, N] (contiguous, out_dtype) = act((a . b^T) * a_scale_m * b_scale_n + bias_n): a [M, K] the tokens, b [N, K] the
- * channels of a weight; bias [N] f32 or NULL; act = max(., 0) with UHM_RELU (NaN stays NaN).  M, N >= 0.
+ * channels of a weight; bias [N] f32 or NULL; act = max(., 0) with UHM_RELU (NaN stays NaN).  M, N >= 0;
+ * out overlaps none of the operands; at most 2^22 blocks of 32 x 64 outputs and 2^27 channels.
  * Few rows: the sum over K is split over blocks and joined in integers through `workspace` (uhm_int8_matmul_workspace_bytes,
  * may be 0 and NULL then; 16-byte aligned).                                                                                  */
 #define UHM_RELU 1u

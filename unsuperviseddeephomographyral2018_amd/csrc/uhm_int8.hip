@@ -10,10 +10,10 @@
 // Few rows leave few tiles (fc1 at 64 pairs: 16 of 64 x 64): the K range is split over blocks, each writes its 32-bit sums to the
 // workspace, and int8_join_kernel adds them (integers: the split does not change the result) and applies the epilogue.
 //
-// Measured on one MI355X (launches of three sets of operands in turn, so that the weight comes from memory):
-//   fc1, 1024 x 32768:  1 pair 9.7 us (3.5 TB/s), from float 11.1; 64 pairs 13.0; 128 pairs from float 22 (quantising 6, product 11, join 4)
-//   4096 x 4096 x 8192: 147 us; each 8192 of K more take 115 us = 2.4 POP/s.  Its loop without loads takes 90 us, with neither loads
-//   nor LDS reads 69 us (the matrix instructions alone, at the clock that their power leaves): no latency is left to hide.
+// Measured on one MI355X (several sets of operands in turn, so that the weight comes from memory; passes among others):
+//   fc1, 1024 x 32768:  1 pair 7.9 us (4.3 TB/s), from float 9.9; 64 pairs 11.0; 128 pairs from float 20.0 (quantising 6, product 11, join 3)
+//   4096 x 4096 x 8192: 134 us with bf16 results; each 8192 of K more take 115 us = 2.4 POP/s.  The loop without loads takes 90 us, with
+//   neither loads nor LDS reads 69 us (the matrix instructions alone, at the clock that their power leaves): power, not latency.
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -47,13 +47,13 @@ __device__ __forceinline__ void put(void* out, int dtype, size_t at, float v) {
     else ((_Float16*)out)[at] = (_Float16)v;
 }
 
-// the first `keep` of 16 bytes, zeros behind them
+// the first `keep` of 4 and of 16 bytes, zeros behind them
+__device__ __forceinline__ unsigned keep_first(unsigned w, int keep) {
+    return keep >= 4 ? w : (keep <= 0 ? 0u : w & ((1u << (8 * keep)) - 1u));
+}
 __device__ __forceinline__ v4i keep_first(v4i v, int keep) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int b = keep - 4 * j;                                    // bytes of word j that count
-        v[j] &= b >= 4 ? -1 : (b <= 0 ? 0 : (int)((1u << (8 * b)) - 1u));
-    }
+    for (int j = 0; j < 4; ++j) v[j] = (int)keep_first((unsigned)v[j], keep - 4 * j);
     return v;
 }
 // the 16 bytes of a row from k on, zero behind K (one operand's zeros are enough for the product, the other's bytes may be anything)
@@ -261,17 +261,6 @@ __device__ __forceinline__ unsigned quantise(float x, RowScale s) {
     if (s.inverse == 0.f) return 0;
     return __float_as_uint(fmaf(x, s.inverse, 0x1.8p23f)) & 0xffu;
 }
-struct F4 { float v[4]; };
-__device__ __forceinline__ unsigned quantise4(const F4& x, RowScale s) {
-    return quantise(x.v[0], s) | quantise(x.v[1], s) << 8 | quantise(x.v[2], s) << 16 | quantise(x.v[3], s) << 24;
-}
-__device__ __forceinline__ unsigned top_of(const F4& x) {
-    unsigned t = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) t = max(t, __float_as_uint(x.v[j]) & 0x7fffffffu);
-    return t;
-}
-
 template <int T> struct Raw { using type = unsigned short; };
 template <> struct Raw<UHM_F32> { using type = float; };
 template <int T>
@@ -280,34 +269,39 @@ __device__ __forceinline__ float value(typename Raw<T>::type r) {
     else if constexpr (T == UHM_BF16) return __uint_as_float((unsigned)r << 16);
     else return __half2float(__ushort_as_half(r));
 }
-// Elements k .. k + 3 of a row (k % 4 == 0), zeros behind K.  WHOLE: rows start on four elements and K ends on four; a load has no
-// branch then (past K the last four are given again: they change no maximum, and the caller drops them), so that many are in flight.
-template <int X, bool WHOLE>
-__device__ __forceinline__ F4 load4(const void* row, int k, int K) {
-    using raw = typename Raw<X>::type;
-    struct alignas(4 * sizeof(raw)) R4 { raw v[4]; };
-    F4 x = {{0.f, 0.f, 0.f, 0.f}};
-    if constexpr (WHOLE) {
-        const R4 r = *reinterpret_cast<const R4*>((const raw*)row + min(k, K - 4));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x.v[j] = value<X>(r.v[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (k + j < K) x.v[j] = value<X>(((const raw*)row)[k + j]);
-    }
-    return x;
-}
-// COUNT of them, STEP elements apart
+// Four elements of a row as they are in memory
+template <int X> struct Four { typename Raw<X>::type v[4]; };
+// COUNT times elements k .. k + 3, `step` elements apart.  Rows may start anywhere: the loads ask for no more than an element's
+// alignment.  None has a branch, so that all are in flight: past K they give the row's last four again, which change no maximum.
 template <int X, int COUNT>
-__device__ __forceinline__ void load4s(F4 (&x)[COUNT], const void* row, int k, int step, int K, int whole) {
-    if (whole) {
+__device__ __forceinline__ void load4s(Four<X> (&x)[COUNT], const void* row, int k, int step, int K) {
+    using raw = typename Raw<X>::type;
+    if (K >= 4) {                                                  // (the same for every thread)
 #pragma unroll
-        for (int i = 0; i < COUNT; ++i) x[i] = load4<X, true>(row, k + i * step, K);
+        for (int i = 0; i < COUNT; ++i) x[i] = *reinterpret_cast<const Four<X>*>((const raw*)row + min(k + i * step, K - 4));
     } else {
 #pragma unroll
-        for (int i = 0; i < COUNT; ++i) x[i] = load4<X, false>(row, k + i * step, K);
+        for (int i = 0; i < COUNT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[i].v[j] = ((const raw*)row)[min(j, K - 1)];
     }
+}
+template <int X>
+__device__ __forceinline__ unsigned top_of(const Four<X>& x) {
+    unsigned t = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t = max(t, __float_as_uint(value<X>(x.v[j])) & 0x7fffffffu);
+    return t;
+}
+// elements k .. k + 3 (as load4s read them) in 8 bits, zeros behind K
+template <int X>
+__device__ __forceinline__ unsigned quantise4(const Four<X>& x, int k, int K, RowScale s) {
+    unsigned w = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w |= quantise(value<X>(x.v[j]), s) << (8 * j);
+    const int keep = K - k;                                        // of the group that K ends in, the last `keep` of four were read
+    if (K >= 4 && keep < 4) w = keep <= 0 ? 0u : w >> (8 * (4 - keep));
+    return keep_first(w, keep);
 }
 
 // the largest of `top` over a block of T threads, in every thread
@@ -329,30 +323,30 @@ __device__ __forceinline__ unsigned block_max(unsigned top) {
 // a longer one is read a second time (out of the L2).  All of a thread's loads are in flight together.
 template <int X, int T>
 __global__ __launch_bounds__(T) void quantize_rows_kernel(const void* __restrict__ x, long long x_ld, int8_t* __restrict__ q,
-                                                          long long q_ld, float* __restrict__ scale, int K, int whole) {
+                                                          long long q_ld, float* __restrict__ scale, int K) {
     constexpr int HELD = 8, SEGMENT = HELD * T * 4;
     const size_t row = blockIdx.x;
     const char* px = (const char*)x + row * x_ld * sizeof(typename Raw<X>::type);
     const int padded = (K + 15) & ~15, k0 = threadIdx.x * 4;
-    F4 held[HELD];
+    Four<X> held[HELD];
     unsigned top = 0;
     for (int base = SEGMENT; base < K; base += SEGMENT) {
-        load4s<X>(held, px, base + k0, T * 4, K, whole);
+        load4s<X>(held, px, base + k0, T * 4, K);
 #pragma unroll
         for (int i = 0; i < HELD; ++i) top = max(top, top_of(held[i]));
     }
-    load4s<X>(held, px, k0, T * 4, K, whole);
+    load4s<X>(held, px, k0, T * 4, K);
 #pragma unroll
     for (int i = 0; i < HELD; ++i) top = max(top, top_of(held[i]));
     const RowScale s = row_scale(block_max<T>(top));
     if (threadIdx.x == 0) scale[row] = s.scale;
     int8_t* pq = q + row * q_ld;
     for (int base = 0; base < padded; base += SEGMENT) {
-        if (base) load4s<X>(held, px, base + k0, T * 4, K, whole);
+        if (base) load4s<X>(held, px, base + k0, T * 4, K);
 #pragma unroll
         for (int i = 0; i < HELD; ++i) {
             const int k = base + k0 + i * T * 4;
-            if (k < padded) *reinterpret_cast<unsigned*>(pq + k) = k < K ? quantise4(held[i], s) : 0;
+            if (k < padded) *reinterpret_cast<unsigned*>(pq + k) = quantise4<X>(held[i], k, K, s);
         }
     }
 }
@@ -364,7 +358,7 @@ __global__ __launch_bounds__(T) void quantize_rows_kernel(const void* __restrict
 // of that float type, quantised here: every block finds the row's maximum again (the row comes out of the L2) and keeps AHEAD
 // steps of it in registers until then (what is longer is read again).
 template <int T, int R, int MB, int X>
-__global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x, long long x_ld, int whole, const int8_t* __restrict__ b,
+__global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x, long long x_ld, const int8_t* __restrict__ b,
                                                      long long b_ld, int M, int N, int K, const Epilogue e) {
     static_assert(X < 0 || MB == 1, "one token");
     constexpr int STEP = T * 16, AHEAD = R * MB >= 16 ? 2 : 4;
@@ -379,9 +373,9 @@ __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x,
     // want them would take four times as many cycles per load (fc1: 5 us more) -- and hands them over in LDS, in 8 bits.
     constexpr int SEGMENT = AHEAD * STEP, HELD = X >= 0 ? SEGMENT / (T * 4) : 1;
     __shared__ v4i row8[X >= 0 ? SEGMENT / 16 : 1];
-    F4 held[HELD];
+    Four<(X < 0 ? UHM_F32 : X)> held[HELD];
     if constexpr (X >= 0) {
-        load4s<X>(held, x, tid * 4, T * 4, K, whole);
+        load4s<X>(held, x, tid * 4, T * 4, K);
         __builtin_amdgcn_sched_barrier(0);
     }
     // loads without a branch: past K the last 16 bytes again, which meet zeros of the token
@@ -402,8 +396,8 @@ __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x,
 #pragma unroll
         for (int i = 0; i < HELD; ++i) top = max(top, top_of(held[i]));
         for (int base = SEGMENT; base < K; base += SEGMENT) {
-            F4 more[HELD];
-            load4s<X>(more, x, base + tid * 4, T * 4, K, whole);
+            Four<X> more[HELD];
+            load4s<X>(more, x, base + tid * 4, T * 4, K);
 #pragma unroll
             for (int i = 0; i < HELD; ++i) top = max(top, top_of(more[i]));
         }
@@ -430,13 +424,13 @@ __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x,
     for (int base = 0; base < K; base += SEGMENT) {
         if constexpr (X >= 0) {
             if (base) {
-                load4s<X>(held, x, base + tid * 4, T * 4, K, whole);      // (again, out of the L2)
+                load4s<X>(held, x, base + tid * 4, T * 4, K);      // (again, out of the L2)
                 __syncthreads();                                   // everyone is through with the segment before
             }
 #pragma unroll
             for (int i = 0; i < HELD; ++i) {
                 const int k = base + (i * T + tid) * 4;
-                reinterpret_cast<unsigned*>(row8)[i * T + tid] = k < K ? quantise4(held[i], s) : 0;
+                reinterpret_cast<unsigned*>(row8)[i * T + tid] = quantise4<X>(held[i], k, K, s);
             }
             __syncthreads();
         }
@@ -489,6 +483,14 @@ constexpr long long FEW = 2;               // tokens up to which int8_few_kernel
 
 struct Plan { int bm, bn, splits, tiles_per_split; };
 
+// The tile by how many of them there are, splits of K where they do not fill the 256 CUs (each measured against every other tile and
+// split on 16 shapes; the rule is within 8 % of the best of each).  us, tile / splits taken | the other side:
+//   32 x 128 up to 32 tokens:  16 x 1024 x 32768 12.2 at 32 splits | 13.8 at 64
+//   256 x 256 from 200 tiles:  4096 x 4096 x 8192 154 | 210 with 128 x 128; below, 1500 x 1500 x 3000 (36 of them) 27 | 56
+//   128 x 128 from 200 tiles:  2048 x 2048 x 2048 23.2 | 24.5 with 64 x 64; below, 1024 x 1024 x 1024 (64 of them) 8.7 | 15.9
+//   64 x 64:                   64 x 1024 x 32768 13.1 at 16 splits | 14.2 at 32, 15.7 at 8; 1000 x 300 x 6000 14.3 at 4 | 17.3 at 8, 18.9 at 1
+// At least 8 tiles of K per split (a block's first loads take as long as several tiles), 4 where there are few blocks anyway:
+// 100 x 50 x 5000 7.8 | 8.8.
 inline Plan plan_of(long long M, long long N, long long K) {
     const auto tiles_of = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
     Plan p;
@@ -496,11 +498,11 @@ inline Plan plan_of(long long M, long long N, long long K) {
     if (M <= 32) { p.bm = 32; p.bn = 128; most = 32; }
     else if (tiles_of(256, 256) >= 200) { p.bm = p.bn = 256; most = 1; }
     else if (tiles_of(128, 128) >= 200) { p.bm = p.bn = 128; most = 1; }
-    else { p.bm = p.bn = 64; most = 16; }
-    const long long tiles = tiles_of(p.bm, p.bn), kt = (K + BK - 1) / BK;
+    else { p.bm = p.bn = 64; most = tiles_of(64, 64) <= 8 ? 32 : 16; }
+    const long long tiles = tiles_of(p.bm, p.bn), kt = (K + BK - 1) / BK, least = tiles <= 16 ? 4 : 8;
     long long s = tiles < 256 ? 512 / tiles : 1;
     if (s > most) s = most;
-    if (s > kt / 8) s = kt / 8;                // at least 8 tiles of K each: a block's first loads take as long as several tiles
+    if (s > kt / least) s = kt / least;
     if (s < 1) s = 1;
     p.tiles_per_split = (int)((kt + s - 1) / s);
     p.splits = (int)((kt + p.tiles_per_split - 1) / p.tiles_per_split);
@@ -510,13 +512,13 @@ inline Plan plan_of(long long M, long long N, long long K) {
 int check_product(long long M, long long N, long long K) {
     if (M < 0 || N < 0 || K < 1) return UHM_E_SHAPE;
     if (K > MAX_K || M > MAX_DIM || N > MAX_DIM) return UHM_E_TOO_LARGE;
-    // the grid is a line of blocks: at most 2^23 tiles (K is only split where they are few)
-    if (((M + 31) / 32) * ((N + 63) / 64) > (1LL << 23)) return UHM_E_TOO_LARGE;
+    // the grid is a line of blocks, fewer than 2^32 threads: at most 2^22 tiles of 32 x 64 (K is only split where they are few)
+    if (N > (1LL << 27) || ((M + 31) / 32) * ((N + 63) / 64) > (1LL << 22)) return UHM_E_TOO_LARGE;
     return 0;
 }
 
 // what the entry points for products check alike (x: the tokens, in 8 bits or as floats)
-int check_operands(const void* x, long long x_ld, const int8_t* b, long long b_ld, const float* b_scale, const float* bias, const void* out,
+int check_operands(const void* x, int x_size, long long x_ld, const int8_t* b, long long b_ld, const float* b_scale, const float* bias, const void* out,
                    int out_dtype, long long M, long long N, long long K, unsigned flags) {
     if (int err = check_product(M, N, K)) return err;
     if (x_ld < K || b_ld < K) return UHM_E_SHAPE;
@@ -527,32 +529,35 @@ int check_operands(const void* x, long long x_ld, const int8_t* b, long long b_l
     if (!x || !b || !b_scale || !out) return UHM_E_NULL;
     if ((((uintptr_t)b | (uintptr_t)b_ld) & 15) || (((uintptr_t)b_scale | (uintptr_t)bias) & 3) || ((uintptr_t)out & (out_dtype == UHM_F32 ? 3 : 1)))
         return UHM_E_ALIGN;
+    const uintptr_t from = (uintptr_t)out, to = from + (uintptr_t)M * N * (out_dtype == UHM_F32 ? 4 : 2);
+    const auto meets = [&](const void* p, uintptr_t bytes) { return p && (uintptr_t)p < to && from < (uintptr_t)p + bytes; };
+    if (meets(x, ((uintptr_t)(M - 1) * x_ld + K) * x_size) || meets(b, (uintptr_t)(N - 1) * b_ld + K) || meets(b_scale, (uintptr_t)N * 4) || meets(bias, (uintptr_t)N * 4))
+        return UHM_E_OVERLAP;
     return 0;
-}
-
-// rows start and end on four elements
-inline int rows_whole(const void* x, int dtype, long long x_ld, long long rows, long long K) {
-    const uintptr_t size = dtype == UHM_F32 ? 4 : 2;
-    return K % 4 == 0 && (((uintptr_t)x | (rows > 1 ? (uintptr_t)x_ld * size : 0)) & (4 * size - 1)) == 0;
 }
 
 template <int X>
 int quantize_rows(const void* x, long long x_ld, int8_t* q, long long q_ld, float* scale, long long rows, long long K, hipStream_t s) {
-    const int al = rows_whole(x, X, x_ld, rows, K);
     // as few threads as hold the row in registers
-    auto launch = [&](auto kernel, int threads) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(threads), 0, s, x, x_ld, q, q_ld, scale, (int)K, al);
+    auto launch = [&](auto kernel, int threads) -> int {
+        const long long most = (1LL << 31) / threads;                  // (a launch has fewer than 2^32 threads)
+        for (long long r = 0; r < rows; r += most) {
+            const long long n = rows - r < most ? rows - r : most;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(threads), 0, s, (const char*)x + (size_t)r * x_ld * sizeof(typename Raw<X>::type), x_ld,
+                               q + (size_t)r * q_ld, q_ld, scale + r, (int)K);
+            if (int err = (int)hipGetLastError()) return err;
+        }
+        return 0;
     };
-    if (K <= 2048) launch(quantize_rows_kernel<X, 64>, 64);
-    else if (K <= 8192) launch(quantize_rows_kernel<X, 256>, 256);
-    else launch(quantize_rows_kernel<X, 1024>, 1024);
-    return (int)hipGetLastError();
+    if (K <= 2048) return launch(quantize_rows_kernel<X, 64>, 64);
+    if (K <= 8192) return launch(quantize_rows_kernel<X, 256>, 256);
+    return launch(quantize_rows_kernel<X, 1024>, 1024);
 }
 
 template <int MB, int X>
-int launch_few(const void* x, long long x_ld, int al, const int8_t* b, long long b_ld, int M, int N, int K, const Epilogue& e, hipStream_t s) {
+int launch_few(const void* x, long long x_ld, const int8_t* b, long long b_ld, int M, int N, int K, const Epilogue& e, hipStream_t s) {
     auto launch = [&](auto kernel, int threads, int R) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(((long long)N + R - 1) / R), (unsigned)((M + MB - 1) / MB)), dim3(threads), 0, s, x, x_ld, al, b, b_ld, M, N, K, e);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(((long long)N + R - 1) / R), (unsigned)((M + MB - 1) / MB)), dim3(threads), 0, s, x, x_ld, b, b_ld, M, N, K, e);
     };
     // threads by K (up to four steps of 16 bytes each, then loops), channels per block by N: at least a block for every CU before a block takes more
     auto rows = [&](auto t) {
@@ -569,8 +574,8 @@ int launch_few(const void* x, long long x_ld, int al, const int8_t* b, long long
 
 int product(const int8_t* a, long long a_ld, const int8_t* b, long long b_ld, long long M, long long N, long long K, const Epilogue& e, int* sums,
             hipStream_t s) {
-    if (M <= 1) return launch_few<1, -1>(a, a_ld, 1, b, b_ld, (int)M, (int)N, (int)K, e, s);
-    if (M <= FEW) return launch_few<2, -1>(a, a_ld, 1, b, b_ld, (int)M, (int)N, (int)K, e, s);
+    if (M <= 1) return launch_few<1, -1>(a, a_ld, b, b_ld, (int)M, (int)N, (int)K, e, s);
+    if (M <= FEW) return launch_few<2, -1>(a, a_ld, b, b_ld, (int)M, (int)N, (int)K, e, s);
     const Plan p = plan_of(M, N, K);
     const int mt = (int)((M + p.bm - 1) / p.bm), nt = (int)((N + p.bn - 1) / p.bn);
     if (p.splits == 1) sums = nullptr;
@@ -640,7 +645,7 @@ extern "C" size_t uhm_int8_matmul_workspace_bytes(long long M, long long N, long
 extern "C" int uhm_int8_matmul(const int8_t* a, long long a_ld, const float* a_scale, const int8_t* b, long long b_ld,
                                const float* b_scale, const float* bias, void* out, int out_dtype, long long M, long long N, long long K,
                                unsigned flags, void* workspace, size_t workspace_bytes, uhm_stream_t stream) {
-    if (int err = check_operands(a, a_ld, b, b_ld, b_scale, bias, out, out_dtype, M, N, K, flags)) return err;
+    if (int err = check_operands(a, 1, a_ld, b, b_ld, b_scale, bias, out, out_dtype, M, N, K, flags)) return err;
     if (M == 0 || N == 0) return 0;
     if (!a_scale) return UHM_E_NULL;
     if (M > 1 && a_ld > MAX_LD) return UHM_E_TOO_LARGE;
@@ -658,16 +663,15 @@ extern "C" size_t uhm_int8_linear_workspace_bytes(long long M, long long N, long
 extern "C" int uhm_int8_linear(const void* x, int dtype, long long x_ld, const int8_t* b, long long b_ld, const float* b_scale,
                                const float* bias, void* out, long long M, long long N, long long K, unsigned flags, void* workspace,
                                size_t workspace_bytes, uhm_stream_t stream) {
-    if (int err = check_operands(x, x_ld, b, b_ld, b_scale, bias, out, dtype, M, N, K, flags)) return err;
+    if (int err = check_operands(x, dtype == UHM_F32 ? 4 : 2, x_ld, b, b_ld, b_scale, bias, out, dtype, M, N, K, flags)) return err;
     if (M == 0 || N == 0) return 0;
     if ((uintptr_t)x & (dtype == UHM_F32 ? 3 : 1)) return UHM_E_ALIGN;
     hipStream_t s = (hipStream_t)stream;
     Epilogue e = {nullptr, b_scale, bias, out, dtype, (flags & UHM_RELU) ? 1 : 0};
     if (M == 1) {
-        const int al = rows_whole(x, dtype, x_ld, 1, K);
-        if (dtype == UHM_F32) return launch_few<1, UHM_F32>(x, x_ld, al, b, b_ld, 1, (int)N, (int)K, e, s);
-        if (dtype == UHM_BF16) return launch_few<1, UHM_BF16>(x, x_ld, al, b, b_ld, 1, (int)N, (int)K, e, s);
-        return launch_few<1, UHM_F16>(x, x_ld, al, b, b_ld, 1, (int)N, (int)K, e, s);
+        if (dtype == UHM_F32) return launch_few<1, UHM_F32>(x, x_ld, b, b_ld, 1, (int)N, (int)K, e, s);
+        if (dtype == UHM_BF16) return launch_few<1, UHM_BF16>(x, x_ld, b, b_ld, 1, (int)N, (int)K, e, s);
+        return launch_few<1, UHM_F16>(x, x_ld, b, b_ld, 1, (int)N, (int)K, e, s);
     }
     const LinearSpace w = linear_space(M, N, K);
     if (int err = check_space(workspace, workspace_bytes, w.total)) return err;

@@ -430,11 +430,11 @@ Tensor int8_linear(const py::object& x, const py::object& weight, const py::obje
 PYBIND11_MODULE(_uhm_torch, m) {
     m.def("abi_version", [] { return uhm_abi_version(); });
     m.def("set_error", [](py::object cls) { error_class = cls.release().ptr(); });
-    m.def("global_norm", &global_norm);
-    m.def("clip_by_global_norm", &clip_by_global_norm);
-    m.def("clip_by_global_norm_", &clip_by_global_norm_);
-    m.def("adam_clip_update_", &adam_clip_update_);
-    m.def("quantize_rows", &quantize_rows);
-    m.def("int8_matmul", &int8_matmul);
-    m.def("int8_linear", &int8_linear);
+    m.def("global_norm", torch::wrap_pybind_function(&global_norm));
+    m.def("clip_by_global_norm", torch::wrap_pybind_function(&clip_by_global_norm));
+    m.def("clip_by_global_norm_", torch::wrap_pybind_function(&clip_by_global_norm_));
+    m.def("adam_clip_update_", torch::wrap_pybind_function(&adam_clip_update_));
+    m.def("quantize_rows", torch::wrap_pybind_function(&quantize_rows));
+    m.def("int8_matmul", torch::wrap_pybind_function(&int8_matmul));
+    m.def("int8_linear", torch::wrap_pybind_function(&int8_linear));
 }
