@@ -92,7 +92,8 @@ UHM_API int uhm_adam_clip_update(float* const* params, const void* const* grads,
 /* Rows of f32 / bf16 / f16 x [rows, K] (row stride x_ld in elements) -> q, scale, symmetric around 0:
  *   top = max |x_r|;  scale = top / 127;  q = round_to_nearest_even(x * (127 / top)), the quotients rounded to f32, the product
  *   exact.  A row whose top is below 2^-120 gets q = 0 and scale 0; one that holds an infinity or NaN gets q = 0 and scale NaN
- *   (every product with it is NaN).  q is written up to K rounded up to 16, zeros behind K.                                    */
+ *   (every product with it is NaN).  q is written up to K rounded up to 16, zeros behind K;
+ *   x, q and scale do not overlap.                                 */
 UHM_API int uhm_quantize_rows(const void* x, int dtype, long long x_ld, int8_t* q, long long q_ld, float* scale, long long rows,
                               long long K, uhm_stream_t stream);
 

@@ -65,3 +65,10 @@ def test_norms_that_overlap_what_is_written_are_refused(lib):
     def adam(use, norm):
         return lib.uhm_adam_clip_update(at(dst), at(src), at(m), at(v), at(n), at(t), 1, 1e-3, 0.9, 0.999, 1e-8, 1, 1.0, 0, use, norm, 1 << 23, big, None)
     assert adam((1 << 24) + 8, 64) == -8 and adam(None, 1 << 25) == -8 and adam(None, 1 << 20) == -8
+
+
+def test_quantiser_refuses_overlaps(lib):
+    def q(x=1 << 20, out=1 << 21, scale=64, rows=4, K=60, q_ld=64):
+        return lib.uhm_quantize_rows(x, 0, 60, out, q_ld, scale, rows, K, None)
+    assert q(out=(1 << 20) + 16) == -8 and q(out=(1 << 20) - 16) == -8 and q(out=(1 << 20) + 944) == -8     # x ends at + 960
+    assert q(scale=(1 << 20) + 8) == -8 and q(scale=(1 << 21) + 252) == -8 and q(scale=(1 << 21) - 4) == -8

@@ -352,19 +352,18 @@ __global__ __launch_bounds__(T) void quantize_rows_kernel(const void* __restrict
 }
 
 // ---- few tokens -----------------------------------------------------------------------------------------------------------------
-// Up to MB tokens per block: bound by the one read of the weight.  A block of T threads owns R channels and all of K (no split, no
+// MB tokens: bound by the one read of the weight.  A block of T threads owns R channels and all of K (no split, no
 // join, one launch): thread t holds bytes 16 t .. 16 t + 15 of every T * 16, AHEAD steps of every channel's row are in flight, products on
 // the 4-way dot instruction (for so few tokens they take less time than the loads).  X < 0: tokens in 8 bits.  X >= 0: ONE token
 // of that float type, quantised here: every block finds the row's maximum again (the row comes out of the L2) and keeps AHEAD
 // steps of it in registers until then (what is longer is read again).
 template <int T, int R, int MB, int X>
 __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x, long long x_ld, const int8_t* __restrict__ b,
-                                                     long long b_ld, int M, int N, int K, const Epilogue e) {
+                                                     long long b_ld, int N, int K, const Epilogue e) {
     static_assert(X < 0 || MB == 1, "one token");
-    constexpr int STEP = T * 16, AHEAD = R * MB >= 16 ? 2 : 4;
+    constexpr int STEP = T * 16, AHEAD = 4;
     const int tid = threadIdx.x;
     const long long n0 = (long long)blockIdx.x * R;
-    const int m0 = blockIdx.y * MB;
     const int8_t* pb[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) pb[r] = b + min(n0 + r, (long long)N - 1) * b_ld;
@@ -404,7 +403,7 @@ __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x,
         s = row_scale(block_max<T>(top));
     } else {
 #pragma unroll
-        for (int m = 0; m < MB; ++m) px[m] = (const int8_t*)x + min(m0 + m, M - 1) * x_ld;
+        for (int m = 0; m < MB; ++m) px[m] = (const int8_t*)x + m * x_ld;
     }
 
     int acc[R][MB];
@@ -467,11 +466,11 @@ __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x,
     if (tid < R * MB) {
         const int r = tid / MB, m = tid % MB;
         const long long n = n0 + r;
-        if (n < N && m0 + m < M) {
+        if (n < N) {
             int v = 0;
 #pragma unroll
             for (int wv = 0; wv < WAVES; ++wv) v += sm[wv][tid];
-            put(e.out, e.dtype, (size_t)(m0 + m) * N + n, finish(v, X >= 0 ? s.scale : e.a_scale[m0 + m], e.b_scale[n], e.bias ? e.bias[n] : 0.f, e.relu));
+            put(e.out, e.dtype, (size_t)m * N + n, finish(v, X >= 0 ? s.scale : e.a_scale[m], e.b_scale[n], e.bias ? e.bias[n] : 0.f, e.relu));
         }
     }
 }
@@ -555,9 +554,9 @@ int quantize_rows(const void* x, long long x_ld, int8_t* q, long long q_ld, floa
 }
 
 template <int MB, int X>
-int launch_few(const void* x, long long x_ld, const int8_t* b, long long b_ld, int M, int N, int K, const Epilogue& e, hipStream_t s) {
+int launch_few(const void* x, long long x_ld, const int8_t* b, long long b_ld, int N, int K, const Epilogue& e, hipStream_t s) {
     auto launch = [&](auto kernel, int threads, int R) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(((long long)N + R - 1) / R), (unsigned)((M + MB - 1) / MB)), dim3(threads), 0, s, x, x_ld, b, b_ld, M, N, K, e);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(((long long)N + R - 1) / R)), dim3(threads), 0, s, x, x_ld, b, b_ld, N, K, e);
     };
     // threads by K (up to four steps of 16 bytes each, then loops), channels per block by N: at least a block for every CU before a block takes more
     auto rows = [&](auto t) {
@@ -574,8 +573,8 @@ int launch_few(const void* x, long long x_ld, const int8_t* b, long long b_ld, i
 
 int product(const int8_t* a, long long a_ld, const int8_t* b, long long b_ld, long long M, long long N, long long K, const Epilogue& e, int* sums,
             hipStream_t s) {
-    if (M <= 1) return launch_few<1, -1>(a, a_ld, b, b_ld, (int)M, (int)N, (int)K, e, s);
-    if (M <= FEW) return launch_few<2, -1>(a, a_ld, b, b_ld, (int)M, (int)N, (int)K, e, s);
+    if (M == 1) return launch_few<1, -1>(a, a_ld, b, b_ld, (int)N, (int)K, e, s);
+    if (M == FEW) return launch_few<2, -1>(a, a_ld, b, b_ld, (int)N, (int)K, e, s);
     const Plan p = plan_of(M, N, K);
     const int mt = (int)((M + p.bm - 1) / p.bm), nt = (int)((N + p.bn - 1) / p.bn);
     if (p.splits == 1) sums = nullptr;
@@ -631,6 +630,10 @@ extern "C" int uhm_quantize_rows(const void* x, int dtype, long long x_ld, int8_
     if (rows == 0) return 0;
     if (!x || !q || !scale) return UHM_E_NULL;
     if (((uintptr_t)q & 15) || (q_ld & 15) || ((uintptr_t)x & (dtype == UHM_F32 ? 3 : 1)) || ((uintptr_t)scale & 3)) return UHM_E_ALIGN;
+    // (the last row of q is written up to K rounded up to 16)
+    const uintptr_t xb = (uintptr_t)x, xe = xb + ((uintptr_t)(rows - 1) * x_ld + K) * (dtype == UHM_F32 ? 4 : 2), qb = (uintptr_t)q,
+                    qe = qb + (uintptr_t)(rows - 1) * q_ld + (K + 15) / 16 * 16, sb = (uintptr_t)scale, se = sb + (uintptr_t)rows * 4;
+    if ((qb < xe && xb < qe) || (sb < xe && xb < se) || (sb < qe && qb < se)) return UHM_E_OVERLAP;
     hipStream_t s = (hipStream_t)stream;
     if (dtype == UHM_F32) return quantize_rows<UHM_F32>(x, x_ld, q, q_ld, scale, rows, K, s);
     if (dtype == UHM_BF16) return quantize_rows<UHM_BF16>(x, x_ld, q, q_ld, scale, rows, K, s);
@@ -669,9 +672,9 @@ extern "C" int uhm_int8_linear(const void* x, int dtype, long long x_ld, const i
     hipStream_t s = (hipStream_t)stream;
     Epilogue e = {nullptr, b_scale, bias, out, dtype, (flags & UHM_RELU) ? 1 : 0};
     if (M == 1) {
-        if (dtype == UHM_F32) return launch_few<1, UHM_F32>(x, x_ld, b, b_ld, 1, (int)N, (int)K, e, s);
-        if (dtype == UHM_BF16) return launch_few<1, UHM_BF16>(x, x_ld, b, b_ld, 1, (int)N, (int)K, e, s);
-        return launch_few<1, UHM_F16>(x, x_ld, b, b_ld, 1, (int)N, (int)K, e, s);
+        if (dtype == UHM_F32) return launch_few<1, UHM_F32>(x, x_ld, b, b_ld, (int)N, (int)K, e, s);
+        if (dtype == UHM_BF16) return launch_few<1, UHM_BF16>(x, x_ld, b, b_ld, (int)N, (int)K, e, s);
+        return launch_few<1, UHM_F16>(x, x_ld, b, b_ld, (int)N, (int)K, e, s);
     }
     const LinearSpace w = linear_space(M, N, K);
     if (int err = check_space(workspace, workspace_bytes, w.total)) return err;
