@@ -1,0 +1,119 @@
+"""GPU: what the operators around the regressor promise at their borders: views that share elements, factors and scales at the ends of
+f32, inputs that ask for a gradient."""
+import math
+
+import pytest
+
+torch = pytest.importorskip('torch')
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope='module')
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip('no HIP device')
+    return torch.device('cuda:0')
+
+
+@pytest.fixture(scope='module')
+def ops(dev):
+    from unsuperviseddeephomographyral2018_amd import ops
+    return ops
+
+
+@pytest.fixture(scope='module')
+def UHError():
+    from unsuperviseddeephomographyral2018_amd._lib import UHError
+    return UHError
+
+
+def gen(dev, seed):
+    return torch.Generator(device=dev).manual_seed(seed)
+
+
+# ---- views that share elements ------------------------------------------------------------------------------------------------
+def views(dev):
+    big = torch.arange(1.0, 1201.0, device=dev).view(30, 40)
+    return big, big.reshape(-1)
+
+
+MEET = {
+    'columns': lambda b, f: [b[:, :4], b[:, 2:6]],
+    'columns, third of three': lambda b, f: [b[:, :4], b[:, 4:8], b[:, 7:9]],
+    'all and columns': lambda b, f: [b, b[:, 1:3]],
+    'columns and all': lambda b, f: [b[:, 1:3], b],
+    'a row and columns': lambda b, f: [b[4], b[:, 39:]],
+    'rows of other steps': lambda b, f: [b[::2], b[1::3]],
+    'elements of other steps': lambda b, f: [f[::2], f[1::3]],
+    'columns and their transpose': lambda b, f: [b[:9, :9], b[:9, :9].t()[1:, :1]],
+    'a diagonal and columns': lambda b, f: [b.diagonal(), b[:, 5:6]],
+    'a window in a window': lambda b, f: [b[3:20, 3:20], b[10:12, 10:12]],
+    'halves of elements': lambda b, f: [b[:, :2], b.view(torch.float16)[:, 3:5]],
+    'itself': lambda b, f: [f.as_strided((10, 10), (7, 2))],
+    'itself, windows': lambda b, f: [f.as_strided((20, 10), (5, 1))],
+}
+APART = {
+    'columns': lambda b, f: [b[:, :4], b[:, 4:6], b[:, 20:]],
+    'rows in turn': lambda b, f: [b[::2], b[1::2]],
+    'rows of other steps': lambda b, f: [b[::2], b[1::4], b[3::4]],
+    'elements in turn': lambda b, f: [f[::3], f[1::3], f[2::3]],
+    'elements of other steps': lambda b, f: [f[::6], f[1::2], f[4::6]],
+    'windows': lambda b, f: [b[:10, :10], b[:10, 10:20], b[10:20, :10], b[10:20, 10:20].t()],
+    'a diagonal and what is above it': lambda b, f: [b.diagonal(), b[0, 1:], b[1, 2:], b.diagonal(1, 0, 1)[5:]],
+    'a column and the rest': lambda b, f: [b[:, 0], b[:, 1:]],
+    'halves of elements': lambda b, f: [b[:, :2], b.view(torch.float16)[:, 4:7]],
+    'steps that miss': lambda b, f: [f.as_strided((8, 3), (30, 7)), f.as_strided((8, 3), (30, 7), 3)],
+    'itself': lambda b, f: [f.as_strided((10, 5), (3, 31))],
+    'nothing': lambda b, f: [b[:, :3], b[:, 2:2], b[:0, ::2]],
+}
+
+
+def same_memory(big, ts):
+    """How often each byte of `big` belongs to the views: counted on the host, element by element."""
+    start = big.data_ptr()
+    at = []
+    for t in ts:
+        off = torch.zeros((), dtype=torch.int64)
+        for n, s in zip(t.shape, t.stride()):
+            off = off[..., None] + torch.arange(n) * s
+        first = off.reshape(-1) * t.element_size() + (t.data_ptr() - start)
+        at += [first + k for k in range(t.element_size())]
+    return int(torch.bincount(torch.cat(at), minlength=1).max())
+
+
+@pytest.mark.parametrize('make', MEET.values(), ids=MEET.keys())
+def test_views_that_share_elements_are_refused(ops, dev, UHError, make):
+    big, flat = views(dev)
+    ts = make(big, flat)
+    assert same_memory(big, ts) > 1
+    kept, version = big.clone(), big._version
+    with pytest.raises(UHError, match='twice|OVERLAP'):
+        ops.clip_by_global_norm_(ts, 1.0)
+    assert torch.equal(big, kept) and big._version == version
+    with pytest.raises(UHError, match='twice|OVERLAP'):
+        ops.clip_by_global_norm_(ts[::-1], 1.0)
+    assert torch.equal(big, kept)
+
+
+@pytest.mark.parametrize('make', APART.values(), ids=APART.keys())
+def test_views_that_interleave_are_clipped(ops, dev, make):
+    big, flat = views(dev)
+    ts = make(big, flat)
+    assert same_memory(big, ts) == 1
+    if any(t.dtype == torch.float16 for t in ts):
+        ts[1].fill_(2.0)
+    kept = big.clone()
+    n = math.sqrt(math.fsum(float((t.double() ** 2).sum()) for t in ts))
+    want = [t.double() / n for t in ts]
+    inside = torch.zeros_like(big, dtype=torch.bool).reshape(-1).as_strided(big.shape, big.stride())
+    told = ops.clip_by_global_norm_(ts, 1.0)
+    assert abs(float(told) - n) <= 1.01 * U * n
+    for t, w in zip(ts, want):
+        h = torch.finfo(t.dtype).eps / 2
+        assert bool(((t.double() - w).abs() <= w.abs() * (3 * U + h) * 1.01 + (2.0 ** -25 if t.dtype == torch.float16 else 0)).all())
+    if all(t.dtype == torch.float32 for t in ts):                          # what lies between the views stays
+        for t in ts:
+            inside.as_strided(t.shape, t.stride(), t.storage_offset()).fill_(True)
+        assert torch.equal(big[~inside], kept[~inside])

@@ -8,8 +8,10 @@
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <c10/util/SmallVector.h>
 #include <algorithm>
 #include <deque>
+#include <numeric>
 #include <string>
 #include <vector>
 #include "../../include/uh_model_ops.h"
@@ -228,22 +230,113 @@ py::tuple clip_by_global_norm(const py::object& tensors, double clip_norm, const
     return py::make_tuple(given_back, norm);
 }
 
+// ---- views that are written in place ------------------------------------------------------------------------------------------
+// A view is the bytes base + sum_k stride_k i_k + (0 .. width - 1), 0 <= i_k < size_k.  Whether two views share a byte is whether a sum of
+// terms c x, lo <= x <= hi, reaches an interval.
+struct Term { int64_t c, lo, hi; };                  // c > 0
+using Terms = c10::SmallVector<Term, 8>;             // (300 slices of one tensor are 45000 pairs)
+
+struct Sum {
+    Terms t;                                         // largest c first, each c once
+    c10::SmallVector<int64_t, 9> low, high;          // of the terms from k on
+    int budget = 1 << 16;                            // steps of the search; past them the views count as sharing
+
+    explicit Sum(Terms terms) {
+        std::sort(terms.begin(), terms.end(), [](const Term& a, const Term& b) { return a.c > b.c; });
+        for (const Term& x : terms) {
+            if (!t.empty() && t.back().c == x.c) { t.back().lo += x.lo; t.back().hi += x.hi; }
+            else t.push_back(x);
+        }
+        low.assign(t.size() + 1, 0);
+        high.assign(t.size() + 1, 0);
+        for (size_t k = t.size(); k-- > 0;) {
+            low[k] = low[k + 1] + t[k].c * t[k].lo;
+            high[k] = high[k + 1] + t[k].c * t[k].hi;
+        }
+    }
+    static int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }      // b > 0
+
+    bool search(size_t k, int64_t from, int64_t to) {
+        if (k == t.size()) return from <= 0 && 0 <= to;
+        const int64_t c = t[k].c, first = std::max(t[k].lo, -floor_div(high[k + 1] - from, c)), last = std::min(t[k].hi, floor_div(to - low[k + 1], c));
+        for (int64_t x = first; x <= last; ++x)
+            if (--budget < 0 || search(k + 1, from - c * x, to - c * x)) return true;
+        return false;
+    }
+    bool reaches(int64_t from, int64_t to) {
+        // the terms up to k add up to a multiple of their common divisor, the others to something in [low, high]: rows and columns of one
+        // larger tensor are told apart here
+        int64_t g = 0;
+        for (size_t k = 0; k < t.size(); ++k) {
+            g = std::gcd(g, t[k].c);
+            if (floor_div(to - low[k + 1], g) * g < from - high[k + 1]) return false;
+        }
+        return search(0, from, to);
+    }
+};
+
+struct View {
+    uintptr_t base, end;
+    int64_t width, row = 0, rows = 0, within;        // the largest stride, the bytes it spans, and those that the rest spans
+    c10::SmallVector<std::pair<int64_t, int64_t>, 4> dims;             // stride in bytes, size - 1
+    bool copied;                                     // clipped in a copy: the native check sees the copy
+    explicit View(const Tensor& v)
+        : base((uintptr_t)v.data_ptr()), end(base + v.element_size()), width(v.element_size()), copied(v.is_neg() || !v.is_non_overlapping_and_dense()) {
+        for (int64_t i = 0; i < v.dim(); ++i) {
+            const int64_t stride = v.stride(i) * width, last = v.size(i) - 1;
+            if (last < 1) continue;
+            dims.push_back({stride, last});
+            end += stride * last;
+            if (stride > row) { row = stride; rows = stride * last; }
+        }
+        within = (int64_t)(end - base) - rows;
+    }
+    bool shares(const View& o) const {
+        const int64_t gap = (int64_t)(o.base - base);
+        if (row && row == o.row && gap >= 0 && gap % row >= within && gap % row + o.within <= row) return false;      // other columns of the same rows
+        Terms terms;
+        for (const auto& d : dims) terms.push_back({d.first, 0, d.second});
+        for (const auto& d : o.dims) terms.push_back({d.first, -d.second, 0});
+        return Sum(std::move(terms)).reaches(gap - (width - 1), gap + (o.width - 1));
+    }
+    bool shares_with_itself() const {                // two indexes, apart first in dimension k, for one byte
+        for (size_t k = 0; k < dims.size(); ++k) {
+            Terms terms = {{dims[k].first, 1, dims[k].second}};
+            for (size_t j = k + 1; j < dims.size(); ++j) terms.push_back({dims[j].first, -dims[j].second, dims[j].second});
+            if (Sum(std::move(terms)).reaches(-(width - 1), width - 1)) return true;
+        }
+        return false;
+    }
+};
+
+// whether an element of a view that is clipped in a copy is given twice (among tensors without gaps the native call checks that)
+bool shares_elements(const vector<const Tensor*>& ts) {
+    if (std::none_of(ts.begin(), ts.end(), [](const Tensor* t) { return t->is_neg() || !t->is_non_overlapping_and_dense(); })) return false;
+    vector<View> v;
+    v.reserve(ts.size());
+    for (const Tensor* t : ts)
+        if (t->numel()) v.emplace_back(*t);
+    std::sort(v.begin(), v.end(), [](const View& a, const View& b) { return a.base < b.base; });
+    for (size_t i = 0; i < v.size(); ++i) {
+        if (v[i].copied && v[i].shares_with_itself()) return true;
+        for (size_t j = i + 1; j < v.size() && v[j].base < v[i].end; ++j)
+            if ((v[i].copied || v[j].copied) && v[i].shares(v[j])) return true;
+    }
+    return false;
+}
+
 Tensor clip_by_global_norm_(const py::object& tensors, double clip_norm, const py::object& use) {
     const char* name = "clip_by_global_norm_";
     clip_value(clip_norm, name);
     List l = take_list(tensors, "tensors", false);
     const vector<const Tensor*> given = l.t;
     const Tensor use_norm = given_norm(use, l.device, name);
-    vector<const void*> strided;
     for (const Tensor* t : given) {
         no_gradient(*t, name);
-        if (!t->is_neg() && t->is_non_overlapping_and_dense()) continue;
-        for (int64_t i = 0; i < t->dim(); ++i)                          // slices of something larger: clipped in a copy
+        for (int64_t i = 0; i < t->dim() && t->numel(); ++i)            // slices of something larger: clipped in a copy
             if (t->stride(i) == 0 && t->size(i) > 1) fail(string(name) + ": an expanded tensor cannot be written in place");
-        if (t->numel()) strided.push_back(t->data_ptr());
     }
-    std::sort(strided.begin(), strided.end());
-    if (std::adjacent_find(strided.begin(), strided.end()) != strided.end()) fail(string(name) + ": the same elements are given twice");
+    if (shares_elements(given)) fail(string(name) + ": the same elements are given twice (views that overlap)");
     const Call call(l.device);
     l.make_dense();
     const Tensor norm = clip(call, Described(l), pointers(l), clip_norm, use_norm, name);

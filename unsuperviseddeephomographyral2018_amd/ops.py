@@ -738,8 +738,10 @@ def clip_by_global_norm(tensors, clip_norm, use_norm=None):
 
 
 def clip_by_global_norm_(tensors, clip_norm, use_norm=None):
-    """clip_by_global_norm in place -> norm.  When nothing has to be clipped, nothing is written.  A tensor that is given twice,
-    tensors that overlap, and expanded ones are refused.  Can be captured into a hipGraph."""
+    """clip_by_global_norm in place -> norm.  When nothing has to be clipped, the values stay (tensors without gaps are then not
+    written; views of something larger are clipped in a copy that is copied back).  Refused: a tensor that is given twice, tensors
+    and views that share elements (slices that interleave are fine; two of irregular steps whose elements a bounded search cannot
+    tell apart count as sharing), and expanded ones.  Can be captured into a hipGraph."""
     return _lib.load_torch_ops().clip_by_global_norm_(tensors, clip_norm, use_norm)
 
 
