@@ -117,3 +117,41 @@ def test_views_that_interleave_are_clipped(ops, dev, make):
         for t in ts:
             inside.as_strided(t.shape, t.stride(), t.storage_offset()).fill_(True)
         assert torch.equal(big[~inside], kept[~inside])
+
+
+# ---- the ends of f32 ------------------------------------------------------------------------------------------------------------
+FAR = [(1e37, 1e-3), (1e37, 3.9), (1e30, 1e-37), (1e36, 1e-10), (1e37, 2.0 ** -149), (1.0, 1e-40)]
+
+
+def f32(x):
+    return float(torch.tensor(x, dtype=torch.float64).float())
+
+
+@pytest.mark.parametrize('offset', [0, 1])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize('size,clip', FAR)
+def test_clipping_by_factors_below_the_normal_range(ops, dev, size, clip, dtype, offset):
+    """Norm, quotient and product are rounded once each (u), the type once (h); what leaves the normal range is off by a step of 2^-149,
+    bf16's by half of one of 2^-133, and a quotient of a clip that is itself below 2^-124 by as much (2^128 2^-150 2^-126 = 2^-148)."""
+    ts = [(torch.randn(n + offset, generator=gen(dev, n), device=dev) * size).to(dtype)[offset:] for n in (1, 37, 100)]
+    n = math.sqrt(math.fsum(float((t.double() ** 2).sum()) for t in ts))
+    f = f32(clip) / n
+    h = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    edge = 2.0 ** -148 + 2.0 ** -149 + (2.0 ** -134 if h else 0.0)
+    out, told = ops.clip_by_global_norm(ts, clip)
+    assert abs(float(told) - n) <= 1.01 * U * n
+    for t, o in zip(ts, out):
+        assert bool(((o.double() - t.double() * f).abs() <= (t.double() * f).abs() * (3 * U + h) * 1.01 + edge).all())
+    ops.clip_by_global_norm_(ts, clip)
+    assert all(torch.equal(a, b) for a, b in zip(ts, out))
+
+
+def test_adam_with_a_factor_below_the_normal_range(ops, dev):
+    g = torch.randn(5000, generator=gen(dev, 1), device=dev) * 1e36
+    p, m, v = (torch.zeros_like(g) for _ in range(3))
+    n = math.sqrt(float((g.double() ** 2).sum()))
+    ops.adam_clip_update_([p], [g], [m], [v], lr=1e-2, clip_norm=1e-2)
+    want = g.double() * (f32(1e-2) / n)
+    # (1 - beta1) g': the factor 2 u, both products and the constant u each; the squares twice that of g' and u for each of three more
+    assert bool(((m.double() - 0.1 * want).abs() <= (0.1 * want).abs() * 5 * U * 1.01).all())
+    assert bool(((v.double() - 0.001 * want ** 2).abs() <= (0.001 * want ** 2) * 9 * U * 1.01).all())

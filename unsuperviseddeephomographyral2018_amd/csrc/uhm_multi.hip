@@ -183,23 +183,33 @@ __global__ __launch_bounds__(THREADS) void finish_norm_kernel(const double* __re
     if (threadIdx.x == 0) norm[0] = n;
 }
 
-__device__ __forceinline__ float clip_factor(float n, float clip) {
-    if (!(n < INFINITY)) return __builtin_nanf("");      // inf or NaN (a norm is never negative)
-    return n > clip ? clip / n : 1.0f;
+// f as a product first * rest.  A quotient below 2^-126 would keep few of its bits in f32 (3e38 clipped to 1e-3: 2e-4 off): it is kept 2^126
+// times as large (clip < 4 there, so that nothing overflows) and rest, otherwise 1, takes that back, exactly.
+struct Factor {
+    float first, rest;
+    __device__ __forceinline__ float operator()(float x) const { return x * first * rest; }
+    __device__ __forceinline__ bool changes_nothing() const { return first == 1.0f && rest == 1.0f; }
+};
+__device__ __forceinline__ Factor clip_factor(float n, float clip) {
+    if (!(n < INFINITY)) return {__builtin_nanf(""), 1.0f};      // inf or NaN (a norm is never negative)
+    if (!(n > clip)) return {1.0f, 1.0f};
+    const float f = clip / n;
+    if (f >= 0x1p-126f) return {f, 1.0f};
+    return {clip * 0x1p126f / n, 0x1p-126f};
 }
 
 template <int T, bool STREAM>
-__device__ __forceinline__ void scale(const void* p, void* out, float f, long long begin, long long end, bool aligned) {
+__device__ __forceinline__ void scale(const void* p, void* out, const Factor f, long long begin, long long end, bool aligned) {
     const auto* q = (const typename Type<T>::raw*)p;
     auto* o = (typename Type<T>::raw*)out;
     over_chunk<Vec<T>::N>(begin, end, aligned,
         [&](long long i) {
             Vec<T> x = *reinterpret_cast<const Vec<T>*>(q + i);
 #pragma unroll
-            for (int e = 0; e < Vec<T>::N; ++e) x.v[e] = Type<T>::put(Type<T>::get(x.v[e]) * f);   // one rounding to the type
+            for (int e = 0; e < Vec<T>::N; ++e) x.v[e] = Type<T>::put(f(Type<T>::get(x.v[e])));   // one rounding to the type
             store<STREAM>(reinterpret_cast<Vec<T>*>(o + i), x);
         },
-        [&](long long i) { o[i] = Type<T>::put(Type<T>::get(q[i]) * f); });
+        [&](long long i) { o[i] = Type<T>::put(f(Type<T>::get(q[i]))); });
 }
 
 // The order of a table's chunks in the second pass.  STREAM: lists that the caches do not hold.  The last tensors that the first
@@ -214,12 +224,12 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(const ClipTable t, const
                                                         const float* __restrict__ use_norm, float clip, float* __restrict__ norm) {
     const float n = use_norm ? use_norm[0] : norm_of(partial, count);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = n;
-    const float f = clip_factor(n, clip);
+    const Factor f = clip_factor(n, clip);
     for (unsigned c = blockIdx.x; c < t.chunks; c += gridDim.x) {
         const Part h = find(t, in_order<STREAM>(c, t.chunks));
         const void* p = t.p[0][h.tensor];
         void* o = t.p[1][h.tensor];
-        if (p == o && f == 1.0f) continue;               // in place and nothing to clip: the values are there
+        if (p == o && f.changes_nothing()) continue;               // in place and nothing to clip: the values are there
         switch (h.type) {
             case UHM_F32: scale<UHM_F32, STREAM>(p, o, f, h.begin, h.end, h.aligned); break;
             case UHM_BF16: scale<UHM_BF16, STREAM>(p, o, f, h.begin, h.end, h.aligned); break;
@@ -237,7 +247,7 @@ __device__ __forceinline__ void adam_one(float& p, float g, float& m, float& v, 
 }
 
 template <int T, bool STREAM>
-__device__ __forceinline__ void adam(float* p, const void* grad, float* m, float* v, float f, const AdamScalars& a, long long begin,
+__device__ __forceinline__ void adam(float* p, const void* grad, float* m, float* v, const Factor f, const AdamScalars& a, long long begin,
                                      long long end, bool aligned) {
     const auto* g = (const typename Type<T>::raw*)grad;
     struct alignas(sizeof(typename Type<T>::raw) * 4) G4 { typename Type<T>::raw v[4]; };
@@ -246,15 +256,15 @@ __device__ __forceinline__ void adam(float* p, const void* grad, float* m, float
             float4 pp = fetch<STREAM>(reinterpret_cast<const float4*>(p + i)), mm = fetch<STREAM>(reinterpret_cast<const float4*>(m + i)),
                    vv = fetch<STREAM>(reinterpret_cast<const float4*>(v + i));
             const G4 gg = *reinterpret_cast<const G4*>(g + i);
-            adam_one(pp.x, Type<T>::get(gg.v[0]) * f, mm.x, vv.x, a);
-            adam_one(pp.y, Type<T>::get(gg.v[1]) * f, mm.y, vv.y, a);
-            adam_one(pp.z, Type<T>::get(gg.v[2]) * f, mm.z, vv.z, a);
-            adam_one(pp.w, Type<T>::get(gg.v[3]) * f, mm.w, vv.w, a);
+            adam_one(pp.x, f(Type<T>::get(gg.v[0])), mm.x, vv.x, a);
+            adam_one(pp.y, f(Type<T>::get(gg.v[1])), mm.y, vv.y, a);
+            adam_one(pp.z, f(Type<T>::get(gg.v[2])), mm.z, vv.z, a);
+            adam_one(pp.w, f(Type<T>::get(gg.v[3])), mm.w, vv.w, a);
             store<STREAM>(reinterpret_cast<float4*>(p + i), pp);
             store<STREAM>(reinterpret_cast<float4*>(m + i), mm);
             store<STREAM>(reinterpret_cast<float4*>(v + i), vv);
         },
-        [&](long long i) { adam_one(p[i], Type<T>::get(g[i]) * f, m[i], v[i], a); });
+        [&](long long i) { adam_one(p[i], f(Type<T>::get(g[i])), m[i], v[i], a); });
 }
 
 template <bool STREAM>
@@ -264,7 +274,7 @@ __global__ __launch_bounds__(THREADS) void adam_kernel(const AdamTable t, const 
     const float n = use_norm ? use_norm[0] : norm_of(partial, count);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = n;
     if (skip_nonfinite && !(n < INFINITY)) return;
-    const float f = clip_factor(n, clip);
+    const Factor f = clip_factor(n, clip);
     for (unsigned c = blockIdx.x; c < t.chunks; c += gridDim.x) {
         const Part h = find(t, in_order<STREAM>(c, t.chunks));
         const int i = h.tensor;
