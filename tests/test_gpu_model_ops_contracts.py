@@ -155,3 +155,46 @@ def test_adam_with_a_factor_below_the_normal_range(ops, dev):
     # (1 - beta1) g': the factor 2 u, both products and the constant u each; the squares twice that of g' and u for each of three more
     assert bool(((m.double() - 0.1 * want).abs() <= (0.1 * want).abs() * 5 * U * 1.01).all())
     assert bool(((v.double() - 0.001 * want ** 2).abs() <= (0.001 * want ** 2) * 9 * U * 1.01).all())
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize('M', [1, 2, 5, 40, 300])                           # few tokens, tiles with and without a join
+def test_products_of_large_rows_stay_in_range(ops, dev, M, dtype):
+    """Sums times the tokens' scale are past 2^128, times the channels' small scale they are not: one rounding each, as ever."""
+    g = gen(dev, M)
+    x = ((torch.rand(M, 8192, generator=g, device=dev) + 0.5) * 1e36).to(dtype)
+    W = (torch.rand(70, 8192, generator=g, device=dev) + 0.5) * 1e-6
+    w, ws = ops.quantize_rows(W)
+    q, s = ops.quantize_rows(x)
+    sums = q.double() @ w.double().t().contiguous()
+    assert float((sums * s.double()[:, None]).abs().min()) > 2.0 ** 128
+    want = sums * s.double()[:, None] * ws.double()
+    h = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    for y in (ops.int8_linear(x, w, ws), ops.int8_matmul(q, s, w, ws, out_dtype=dtype), ops.int8_matmul(q, -s, w, -ws, out_dtype=dtype)):
+        assert bool(((y.double() - want).abs() <= want * (3 * U + h) * 1.01).all())
+    assert bool((ops.int8_matmul(q, s, w, ws * 1e30) == math.inf).all())   # (a result past the range is infinite)
+
+
+def test_products_with_scales_at_the_ends(ops, dev):
+    """Every combination of large and small scales, against 64 bits: one rounding for each factor."""
+    a, b = torch.full((6, 40), 100, dtype=torch.int8, device=dev), torch.full((6, 40), 100, dtype=torch.int8, device=dev)
+    s = torch.tensor([2.0 ** 120, 2.0 ** 96, 1.5 * 2.0 ** 96, 1.0, 2.0 ** -100, 2.0 ** -126], device=dev)
+    want = (400000.0 * s.double()[:, None]) * s.double()
+    y = ops.int8_matmul(a, s, b, s).double()
+    inside = want < 2.0 ** 127.9
+    assert bool((y[~inside] == math.inf).all())
+    assert bool(((y - want).abs()[inside] <= want[inside] * 3 * U * 1.01 + 2.0 ** -149).all())
+
+
+@pytest.mark.parametrize('M,N,K', [(2000, 1700, 300), (3700, 3650, 127), (33, 129, 4096), (700, 300, 129), (2, 5, 77)])
+def test_some_rows_with_large_scales(ops, dev, M, N, K):
+    """Powers of two: exact.  Only a few rows are large, in some tiles, waves and groups of rows."""
+    a = torch.randint(-128, 128, (M, K), generator=gen(dev, M), device=dev, dtype=torch.int8)
+    b = torch.randint(-128, 128, (N, K), generator=gen(dev, N), device=dev, dtype=torch.int8)
+    sa = torch.ones(M, device=dev)
+    sa[torch.tensor([0, 1, M // 3, M // 2, M - 1], device=dev)] = 2.0 ** 122
+    sb = torch.full((N,), 2.0 ** -20, device=dev)
+    sb[::3] = 2.0 ** -110
+    want = (a.double() @ b.double().t().contiguous()).float().double() * sa.double()[:, None] * sb.double()
+    y = ops.int8_matmul(a, sa, b, sb)
+    assert bool(torch.isfinite(want.float()).all()) and torch.equal(y, want.float())

@@ -36,10 +36,16 @@ struct Epilogue {
     int relu;
 };
 
-// f32 of the integer sum (at most 2^31: one rounding), the two scales one after the other (their product alone could underflow)
-__device__ __forceinline__ float finish(int acc, float sa, float sb, float bias, int relu) {
-    const float v = (float)acc * sa * sb + bias;
+// f32 of the integer sum (at most 2^31: one rounding), the two scales one after the other (their product alone could underflow).  The sum
+// times a token's scale above LARGE could leave f32 where the result does not: there the channel's goes first.
+constexpr float LARGE = 0x1p96f;
+__device__ __forceinline__ float finish_in_order(int acc, float first, float second, float bias, int relu) {
+    const float v = (float)acc * first * second + bias;
     return relu && v < 0.f ? 0.f : v;      // NaN stays
+}
+__device__ __forceinline__ float finish(int acc, float sa, float sb, float bias, int relu) {
+    const bool large = fabsf(sa) > LARGE;
+    return finish_in_order(acc, large ? sb : sa, large ? sa : sb, bias, relu);
 }
 __device__ __forceinline__ void put(void* out, int dtype, size_t at, float v) {
     if (dtype == UHM_F32) ((float*)out)[at] = v;
@@ -218,13 +224,20 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void int8_matmul_kernel(const int8
                 at += 8 * (size_t)N;
             }
     };
+    // (whether a wave has a large scale among its rows is asked once: the choice at every output took 3 % of 2048 x 2048 x 2048)
+    bool large = false;
+    if (!sums)
+#pragma unroll
+        for (int r = 0; r < BM / WM; r += 64) large |= __any(fabsf(scales[wm + min(r + lane, BM / WM - 1)]) > LARGE);
     if (sums) {
         int* part = sums + (size_t)at.z * M * N;
         each([&](size_t at, int v, float, float, float) { part[at] = v; });
-    } else if (e.dtype == UHM_F32) {
-        each([&](size_t at, int v, float sam, float sbn, float bias) { ((float*)e.out)[at] = finish(v, sam, sbn, bias, e.relu); });
-    } else {
+    } else if (large) {
         each([&](size_t at, int v, float sam, float sbn, float bias) { put(e.out, e.dtype, at, finish(v, sam, sbn, bias, e.relu)); });
+    } else if (e.dtype == UHM_F32) {
+        each([&](size_t at, int v, float sam, float sbn, float bias) { ((float*)e.out)[at] = finish_in_order(v, sam, sbn, bias, e.relu); });
+    } else {
+        each([&](size_t at, int v, float sam, float sbn, float bias) { put(e.out, e.dtype, at, finish_in_order(v, sam, sbn, bias, e.relu)); });
     }
 }
 
