@@ -529,9 +529,9 @@ int check_product(long long M, long long N, long long K) {
     return 0;
 }
 
-// what the entry points for products check alike (x: the tokens, in 8 bits or as floats)
-int check_operands(const void* x, int x_size, long long x_ld, const int8_t* b, long long b_ld, const float* b_scale, const float* bias, const void* out,
-                   int out_dtype, long long M, long long N, long long K, unsigned flags) {
+// what the entry points for products check alike (x: the tokens, in 8 bits with a_scale or as floats without)
+int check_operands(const void* x, int x_size, long long x_ld, const float* a_scale, const int8_t* b, long long b_ld, const float* b_scale, const float* bias,
+                   const void* out, int out_dtype, long long M, long long N, long long K, unsigned flags) {
     if (int err = check_product(M, N, K)) return err;
     if (x_ld < K || b_ld < K) return UHM_E_SHAPE;
     if (N > 1 && b_ld > MAX_LD) return UHM_E_TOO_LARGE;
@@ -543,7 +543,7 @@ int check_operands(const void* x, int x_size, long long x_ld, const int8_t* b, l
         return UHM_E_ALIGN;
     const uintptr_t from = (uintptr_t)out, to = from + (uintptr_t)M * N * (out_dtype == UHM_F32 ? 4 : 2);
     const auto meets = [&](const void* p, uintptr_t bytes) { return p && (uintptr_t)p < to && from < (uintptr_t)p + bytes; };
-    if (meets(x, ((uintptr_t)(M - 1) * x_ld + K) * x_size) || meets(b, (uintptr_t)(N - 1) * b_ld + K) || meets(b_scale, (uintptr_t)N * 4) || meets(bias, (uintptr_t)N * 4))
+    if (meets(x, ((uintptr_t)(M - 1) * x_ld + K) * x_size) || meets(a_scale, (uintptr_t)M * 4) || meets(b, (uintptr_t)(N - 1) * b_ld + K) || meets(b_scale, (uintptr_t)N * 4) || meets(bias, (uintptr_t)N * 4))
         return UHM_E_OVERLAP;
     return 0;
 }
@@ -661,7 +661,7 @@ extern "C" size_t uhm_int8_matmul_workspace_bytes(long long M, long long N, long
 extern "C" int uhm_int8_matmul(const int8_t* a, long long a_ld, const float* a_scale, const int8_t* b, long long b_ld,
                                const float* b_scale, const float* bias, void* out, int out_dtype, long long M, long long N, long long K,
                                unsigned flags, void* workspace, size_t workspace_bytes, uhm_stream_t stream) {
-    if (int err = check_operands(a, 1, a_ld, b, b_ld, b_scale, bias, out, out_dtype, M, N, K, flags)) return err;
+    if (int err = check_operands(a, 1, a_ld, a_scale, b, b_ld, b_scale, bias, out, out_dtype, M, N, K, flags)) return err;
     if (M == 0 || N == 0) return 0;
     if (!a_scale) return UHM_E_NULL;
     if (M > 1 && a_ld > MAX_LD) return UHM_E_TOO_LARGE;
@@ -679,7 +679,7 @@ extern "C" size_t uhm_int8_linear_workspace_bytes(long long M, long long N, long
 extern "C" int uhm_int8_linear(const void* x, int dtype, long long x_ld, const int8_t* b, long long b_ld, const float* b_scale,
                                const float* bias, void* out, long long M, long long N, long long K, unsigned flags, void* workspace,
                                size_t workspace_bytes, uhm_stream_t stream) {
-    if (int err = check_operands(x, dtype == UHM_F32 ? 4 : 2, x_ld, b, b_ld, b_scale, bias, out, dtype, M, N, K, flags)) return err;
+    if (int err = check_operands(x, dtype == UHM_F32 ? 4 : 2, x_ld, nullptr, b, b_ld, b_scale, bias, out, dtype, M, N, K, flags)) return err;
     if (M == 0 || N == 0) return 0;
     if ((uintptr_t)x & (dtype == UHM_F32 ? 3 : 1)) return UHM_E_ALIGN;
     hipStream_t s = (hipStream_t)stream;
