@@ -99,7 +99,8 @@ UHM_API int uhm_quantize_rows(const void* x, int dtype, long long x_ld, int8_t* 
 
 /* out [M, N] (contiguous, out_dtype) = act((a . b^T) * a_scale_m * b_scale_n + bias_n): a [M, K] the tokens, b [N, K] the
  * channels of a weight; bias [N] f32 or NULL; act = max(., 0) with UHM_RELU (NaN stays NaN).  M, N >= 0;
- * out overlaps none of the operands; at most 2^22 blocks of 32 x 64 outputs and 2^27 channels.
+ * out overlaps none of the operands, and what is needed of the workspace neither them nor out; at most 2^22 blocks of 32 x 64
+ * outputs and 2^27 channels.
  * Few rows: the sum over K is split over blocks and joined in integers through `workspace` (uhm_int8_matmul_workspace_bytes,
  * may be 0 and NULL then; 16-byte aligned).                                                                                  */
 #define UHM_RELU 1u

@@ -30,3 +30,41 @@ def test_products_refuse_an_output_over_the_tokens_scales(lib, M):
     assert product(lib, M=M, sa=256 * MB) == OVERLAP
     assert product(lib, M=M, sa=256 * MB + M * 1024 * 4 - 4) == OVERLAP
     assert product(lib, M=M, out=96 * MB + 4 * (M - 1)) == OVERLAP
+
+
+def layer(lib, M=64, N=1024, K=32768, x=64 * MB, b=128 * MB, sb=192 * MB, bias=200 * MB, out=256 * MB, w=512 * MB, nbytes=None, dtype=0):
+    if nbytes is None:
+        nbytes = lib.uhm_int8_linear_workspace_bytes(M, N, K)
+    return lib.uhm_int8_linear(x, dtype, K, b, K, sb, bias, out, M, N, K, 0, w, nbytes, None)
+
+
+def over(begin, size, need):
+    """Workspaces that end just inside a span, lie in it, and begin with its last bytes."""
+    return [begin - need + 16, begin, begin + size // 32 * 16, begin + (size - 1) // 16 * 16]
+
+
+def test_products_refuse_a_workspace_over_anything_else(lib):
+    M, N, K = 64, 1024, 32768
+    need = lib.uhm_int8_matmul_workspace_bytes(M, N, K)
+    assert need > 0
+    for begin, size in ((64 * MB, M * K), (96 * MB, 4 * M), (128 * MB, N * K), (192 * MB, 4 * N), (200 * MB, 4 * N), (256 * MB, 4 * M * N)):
+        for w in over(begin, size, need):
+            assert product(lib, w=w) == OVERLAP, (begin, w)
+    assert product(lib, bias=None, w=256 * MB) == OVERLAP
+
+
+def test_layers_refuse_a_workspace_over_anything_else(lib):
+    M, N, K = 64, 1024, 32768
+    for dtype, size in ((0, 4), (1, 2), (2, 2)):
+        need = lib.uhm_int8_linear_workspace_bytes(M, N, K)
+        for begin, length in ((64 * MB, M * K * size), (128 * MB, N * K), (192 * MB, 4 * N), (200 * MB, 4 * N), (256 * MB, size * M * N)):
+            for w in over(begin, length, need):
+                assert layer(lib, w=w, dtype=dtype) == OVERLAP, (begin, w)
+
+
+def test_products_refuse_missing_workspaces(lib):
+    need = lib.uhm_int8_matmul_workspace_bytes(64, 1024, 32768)
+    assert need > 0
+    assert product(lib, w=None) == -4 and product(lib, nbytes=need - 1) == -4 and product(lib, w=512 * MB + 4) == -9
+    need = lib.uhm_int8_linear_workspace_bytes(64, 1024, 32768)
+    assert layer(lib, w=None) == -4 and layer(lib, nbytes=need - 1) == -4 and layer(lib, w=512 * MB + 4) == -9

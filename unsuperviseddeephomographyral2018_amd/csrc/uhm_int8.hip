@@ -529,9 +529,25 @@ int check_product(long long M, long long N, long long K) {
     return 0;
 }
 
-// what the entry points for products check alike (x: the tokens, in 8 bits with a_scale or as floats without)
+// the memory of a call, to find whether something that is written meets any of it
+struct Memory {
+    uintptr_t begin[6], end[6];
+    int count = 0;
+    void add(const void* p, size_t bytes) {
+        if (!p) return;
+        begin[count] = (uintptr_t)p;
+        end[count++] = (uintptr_t)p + bytes;
+    }
+    bool meets(const void* p, size_t bytes) const {
+        for (int i = 0; i < count; ++i)
+            if (begin[i] < (uintptr_t)p + bytes && (uintptr_t)p < end[i]) return true;
+        return false;
+    }
+};
+
+// what the entry points for products check alike (x: the tokens, in 8 bits with a_scale or as floats without); *all: their operands and output
 int check_operands(const void* x, int x_size, long long x_ld, const float* a_scale, const int8_t* b, long long b_ld, const float* b_scale, const float* bias,
-                   const void* out, int out_dtype, long long M, long long N, long long K, unsigned flags) {
+                   const void* out, int out_dtype, long long M, long long N, long long K, unsigned flags, Memory* all) {
     if (int err = check_product(M, N, K)) return err;
     if (x_ld < K || b_ld < K) return UHM_E_SHAPE;
     if (N > 1 && b_ld > MAX_LD) return UHM_E_TOO_LARGE;
@@ -541,10 +557,14 @@ int check_operands(const void* x, int x_size, long long x_ld, const float* a_sca
     if (!x || !b || !b_scale || !out) return UHM_E_NULL;
     if ((((uintptr_t)b | (uintptr_t)b_ld) & 15) || (((uintptr_t)b_scale | (uintptr_t)bias) & 3) || ((uintptr_t)out & (out_dtype == UHM_F32 ? 3 : 1)))
         return UHM_E_ALIGN;
-    const uintptr_t from = (uintptr_t)out, to = from + (uintptr_t)M * N * (out_dtype == UHM_F32 ? 4 : 2);
-    const auto meets = [&](const void* p, uintptr_t bytes) { return p && (uintptr_t)p < to && from < (uintptr_t)p + bytes; };
-    if (meets(x, ((uintptr_t)(M - 1) * x_ld + K) * x_size) || meets(a_scale, (uintptr_t)M * 4) || meets(b, (uintptr_t)(N - 1) * b_ld + K) || meets(b_scale, (uintptr_t)N * 4) || meets(bias, (uintptr_t)N * 4))
-        return UHM_E_OVERLAP;
+    all->add(x, ((size_t)(M - 1) * x_ld + K) * x_size);
+    all->add(a_scale, (size_t)M * 4);
+    all->add(b, (size_t)(N - 1) * b_ld + K);
+    all->add(b_scale, (size_t)N * 4);
+    all->add(bias, (size_t)N * 4);
+    const size_t written = (size_t)M * N * (out_dtype == UHM_F32 ? 4 : 2);
+    if (all->meets(out, written)) return UHM_E_OVERLAP;
+    all->add(out, written);
     return 0;
 }
 
@@ -625,10 +645,11 @@ LinearSpace linear_space(long long M, long long N, long long K) {
     return w;
 }
 
-int check_space(const void* workspace, size_t bytes, size_t need) {
+int check_space(const void* workspace, size_t bytes, size_t need, const Memory& others) {
     if (!need) return 0;
     if (!workspace || bytes < need) return UHM_E_WORKSPACE;
-    return ((uintptr_t)workspace & 15) ? UHM_E_ALIGN : 0;
+    if ((uintptr_t)workspace & 15) return UHM_E_ALIGN;
+    return others.meets(workspace, need) ? UHM_E_OVERLAP : 0;
 }
 
 }  // namespace uhm
@@ -661,12 +682,13 @@ extern "C" size_t uhm_int8_matmul_workspace_bytes(long long M, long long N, long
 extern "C" int uhm_int8_matmul(const int8_t* a, long long a_ld, const float* a_scale, const int8_t* b, long long b_ld,
                                const float* b_scale, const float* bias, void* out, int out_dtype, long long M, long long N, long long K,
                                unsigned flags, void* workspace, size_t workspace_bytes, uhm_stream_t stream) {
-    if (int err = check_operands(a, 1, a_ld, a_scale, b, b_ld, b_scale, bias, out, out_dtype, M, N, K, flags)) return err;
+    Memory all;
+    if (int err = check_operands(a, 1, a_ld, a_scale, b, b_ld, b_scale, bias, out, out_dtype, M, N, K, flags, &all)) return err;
     if (M == 0 || N == 0) return 0;
     if (!a_scale) return UHM_E_NULL;
     if (M > 1 && a_ld > MAX_LD) return UHM_E_TOO_LARGE;
     if ((((uintptr_t)a | (uintptr_t)a_ld) & 15) || ((uintptr_t)a_scale & 3)) return UHM_E_ALIGN;
-    if (int err = check_space(workspace, workspace_bytes, sums_bytes(M, N, K))) return err;
+    if (int err = check_space(workspace, workspace_bytes, sums_bytes(M, N, K), all)) return err;
     const Epilogue e = {a_scale, b_scale, bias, out, out_dtype, (flags & UHM_RELU) ? 1 : 0};
     return product(a, a_ld, b, b_ld, M, N, K, e, (int*)workspace, (hipStream_t)stream);
 }
@@ -679,7 +701,8 @@ extern "C" size_t uhm_int8_linear_workspace_bytes(long long M, long long N, long
 extern "C" int uhm_int8_linear(const void* x, int dtype, long long x_ld, const int8_t* b, long long b_ld, const float* b_scale,
                                const float* bias, void* out, long long M, long long N, long long K, unsigned flags, void* workspace,
                                size_t workspace_bytes, uhm_stream_t stream) {
-    if (int err = check_operands(x, dtype == UHM_F32 ? 4 : 2, x_ld, nullptr, b, b_ld, b_scale, bias, out, dtype, M, N, K, flags)) return err;
+    Memory all;
+    if (int err = check_operands(x, dtype == UHM_F32 ? 4 : 2, x_ld, nullptr, b, b_ld, b_scale, bias, out, dtype, M, N, K, flags, &all)) return err;
     if (M == 0 || N == 0) return 0;
     if ((uintptr_t)x & (dtype == UHM_F32 ? 3 : 1)) return UHM_E_ALIGN;
     hipStream_t s = (hipStream_t)stream;
@@ -690,7 +713,7 @@ extern "C" int uhm_int8_linear(const void* x, int dtype, long long x_ld, const i
         return launch_few<1, UHM_F16>(x, x_ld, b, b_ld, (int)N, (int)K, e, s);
     }
     const LinearSpace w = linear_space(M, N, K);
-    if (int err = check_space(workspace, workspace_bytes, w.total)) return err;
+    if (int err = check_space(workspace, workspace_bytes, w.total, all)) return err;
     int8_t* q = (int8_t*)workspace;
     float* scale = (float*)((char*)workspace + w.scale);
     if (int err = uhm_quantize_rows(x, dtype, x_ld, q, w.q_ld, scale, M, K, stream)) return err;
