@@ -57,10 +57,10 @@ UHM_API const char* uhm_error_string(int code);
  * A list is `count` >= 1 tensors of numel[i] >= 0 contiguous elements of type dtypes[i], each at least element-aligned (16-byte
  * aligned tensors go faster).  numel[i] == 0 tensors are skipped (their pointer may be NULL).  Up to 2^31 - 1 chunks of 4096
  * elements per list.  Sums of squares are held in f64: no finite f32 list over- or underflows.
- * Workspace: uhm_multi_workspace_bytes(count) bytes, 8-byte aligned.                                                       */
+ * Workspace: uhm_multi_workspace_bytes(count) bytes, 8-byte aligned.  It overlaps neither the tensors nor a norm of the call.   */
 UHM_API size_t uhm_multi_workspace_bytes(int count);
 
-/* norm[0] = sqrt(sum_i sum_j tensors[i][j]^2), f32.  Tensors may overlap each other (each counts).                          */
+/* norm[0] = sqrt(sum_i sum_j tensors[i][j]^2), f32.  Tensors may overlap each other (each counts), norm none of them.        */
 UHM_API int uhm_global_norm(const void* const* tensors, const long long* numel, const int* dtypes, int count, float* norm,
                             void* workspace, size_t workspace_bytes, uhm_stream_t stream);
 
