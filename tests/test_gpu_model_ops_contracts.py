@@ -198,3 +198,65 @@ def test_some_rows_with_large_scales(ops, dev, M, N, K):
     want = (a.double() @ b.double().t().contiguous()).float().double() * sa.double()[:, None] * sb.double()
     y = ops.int8_matmul(a, sa, b, sb)
     assert bool(torch.isfinite(want.float()).all()) and torch.equal(y, want.float())
+
+
+# ---- inputs that ask for a gradient -------------------------------------------------------------------------------------------------
+def calls(ops, dev):
+    """name -> (call on its float arguments, those arguments)"""
+    t = lambda *shape: torch.ones(shape, device=dev)
+    q = torch.ones(4, 32, dtype=torch.int8, device=dev)
+    return {'global_norm': (lambda a, b: ops.global_norm([a, b]), [t(5), t(6)]),
+            'clip_by_global_norm': (lambda a, b, n: ops.clip_by_global_norm([a, b], 1.0, use_norm=n), [t(5), t(6), t()]),
+            'clip_by_global_norm_': (lambda a, b, n: ops.clip_by_global_norm_([a, b], 1.0, use_norm=n), [t(5), t(6), t()]),
+            'adam_clip_update_': (lambda p, g, m, v, n: ops.adam_clip_update_([p], [g], [m], [v], lr=1e-2, use_norm=n), [t(5), t(5), t(5), t(5), t()]),
+            'quantize_rows': (ops.quantize_rows, [t(3, 32)]),
+            'int8_matmul': (lambda s, ws, b: ops.int8_matmul(q, s, q, ws, bias=b), [t(4), t(4), t(4)]),
+            'int8_linear': (lambda x, ws, b: ops.int8_linear(x, q, ws, bias=b), [t(3, 32), t(4), t(4)])}
+
+
+CALLS = ['global_norm', 'clip_by_global_norm', 'clip_by_global_norm_', 'adam_clip_update_', 'quantize_rows', 'int8_matmul', 'int8_linear']
+
+
+@pytest.mark.parametrize('name', CALLS)
+def test_inputs_that_ask_for_a_gradient_are_refused(ops, dev, UHError, name):
+    call, args = calls(ops, dev)[name]
+    for i in range(len(args)):
+        if name == 'adam_clip_update_' and i == 0:
+            continue                                                       # a parameter is a leaf that asks for one
+        some = [a.clone() for a in args]
+        kept = [a.clone() for a in some]
+        some[i].requires_grad_()
+        with pytest.raises(UHError, match=name + '.* has no gradient'):
+            call(*some)
+        assert all(torch.equal(a, k) and a._version == 0 for a, k in zip(some, kept))
+        with torch.no_grad():
+            call(*some)
+
+
+@pytest.mark.parametrize('name', CALLS)
+def test_tangents_are_refused(ops, dev, UHError, name):
+    import torch.autograd.forward_ad as fwd
+    call, args = calls(ops, dev)[name]
+    for i in range(len(args)):
+        some = [a.clone() for a in args]
+        with fwd.dual_level():
+            some[i] = fwd.make_dual(some[i], torch.ones_like(some[i]))
+            with pytest.raises(UHError, match=name + '.* has no gradient'):
+                call(*some)
+            with torch.no_grad(), pytest.raises(UHError, match=name + '.* has no gradient'):
+                call(*some)                                                # no_grad is about the backward pass
+            some[i] = fwd.unpack_dual(some[i]).primal
+            call(*some)
+
+
+def test_parameters_are_leaves_or_plain(ops, dev, UHError):
+    state = lambda: [torch.ones(5, device=dev) for _ in range(3)]
+    p = torch.nn.Parameter(torch.ones(5, device=dev))
+    for q in (p, p.detach()):
+        g, m, v = state()
+        ops.adam_clip_update_([q], [g], [m], [v], lr=1e-2)
+    g, m, v = state()
+    with pytest.raises(UHError, match='has no gradient'):
+        ops.adam_clip_update_([p.view(5)], [g], [m], [v], lr=1e-2)         # the update would be missing from the view's graph
+    with torch.no_grad():
+        ops.adam_clip_update_([p.view(5)], [g], [m], [v], lr=1e-2)

@@ -64,9 +64,21 @@ const Tensor& tensor(const py::object& o, const char* name) {
     return THPVariable_Unpack(o.ptr());
 }
 
+// A call records nothing for autograd, backward or forward: inputs that ask for that are refused rather than cut off in silence.
+void no_tangent(const Tensor& t, const char* name) {
+    if (t._fw_grad(/*level=*/0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        fail(string(name) + " has no gradient: pass the primal of a tensor that carries a forward-mode tangent");
+}
 void no_gradient(const Tensor& t, const char* name) {
+    if (!t.unsafeGetTensorImpl()->autograd_meta()) return;             // (lists of gradients: nothing to ask)
     if (t.requires_grad() && at::GradMode::is_enabled())
         fail(string(name) + " has no gradient: pass detached tensors or call it under torch.no_grad()");
+    no_tangent(t, name);
+}
+// what an optimizer updates in place: leaves may ask for a gradient
+void no_gradient_but_of_leaves(const Tensor& t, const char* name) {
+    if (t.is_leaf()) no_tangent(t, name);
+    else no_gradient(t, name);
 }
 
 // values as memory holds them (a lazy negation is carried out)
@@ -370,6 +382,8 @@ Tensor adam_clip_update_(const py::object& params, const py::object& grads, cons
     const Call call(p.device);
     for (size_t i = 0; i < n; ++i) {
         const Tensor &pi = *p.t[i], &gi = *g.t[i], &mi = *m.t[i], &vi = *v.t[i];
+        no_gradient_but_of_leaves(pi, name);
+        for (const Tensor* t : {&gi, &mi, &vi}) no_gradient(*t, name);
         if (pi.sizes() != gi.sizes() || pi.sizes() != mi.sizes() || pi.sizes() != vi.sizes())
             fail(string(name) + ": shapes " + shape_of(pi) + ", " + shape_of(gi) + ", " + shape_of(mi) + ", " + shape_of(vi));
         if (!pi.is_non_overlapping_and_dense() || !laid_out_alike(pi, mi) || !laid_out_alike(pi, vi) || pi.is_neg() || mi.is_neg() || vi.is_neg())

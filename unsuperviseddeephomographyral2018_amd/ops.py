@@ -751,7 +751,8 @@ def adam_clip_update_(params, grads, exp_avgs, exp_avg_sqs, lr, beta1=0.9, beta2
     -> norm.  params, exp_avgs, exp_avg_sqs: float32, updated in place; grads: float32 / bfloat16 / float16, only read; the four
     lists in the same order and shapes; params and moments dense and laid out alike.  step counts from 1.  clip_norm may be inf
     (the norm is then only told).  use_norm: a norm computed before, for lists that are part of a larger one.  A norm that is not
-    finite makes params and moments NaN, or with skip_nonfinite leaves them as they are.  Can be captured into a hipGraph (with the
+    finite makes params and moments NaN, or with skip_nonfinite leaves them as they are.  No gradient: only params that are leaves may
+    ask for one.  Can be captured into a hipGraph (with the
     scalars of that call)."""
     return _lib.load_torch_ops().adam_clip_update_(params, grads, exp_avgs, exp_avg_sqs, lr, beta1, beta2, eps, int(step), clip_norm, use_norm,
                                                    bool(skip_nonfinite))
