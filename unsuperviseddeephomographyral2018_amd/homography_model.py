@@ -64,7 +64,7 @@ class VGGRegressor(nn.Module):
         self.dropout_p = dropout_p
         # conv GEMMs on stock MIOpen; bias + ReLU (+ their backward and the bias gradient) as one HIP pass each
         self.fused_epilogue = fused_epilogue
-        self._int8_fc1 = None                        # (weight, scales, bias) within int8_head()
+        self._int8_fc1 = None                        # within int8_head(): [(columns, weight, scales)]
         chans = [(2, 64), (64, 64), (64, 64), (64, 64), (64, 128), (128, 128), (128, 128), (128, 128)]
         self.convs = nn.ModuleList([nn.Conv2d(i, o, 3, stride=1, padding=1) for i, o in chans])
         self.use_batch_norm = use_batch_norm
@@ -99,9 +99,17 @@ class VGGRegressor(nn.Module):
     @contextlib.contextmanager
     def int8_head(self):
         """Within it, evaluation computes fc1 in 8-bit integers (ops.int8_linear).  The weight is quantised on entry, one scale per
-        channel, and read as 33 MB instead of 134; training mode stays in float32.  No gradient: call under torch.no_grad()."""
-        w, scale = ops.quantize_rows(self.fc1.weight.detach())
-        self._int8_fc1, before = (w, scale, self.fc1.bias.detach()), self._int8_fc1
+        channel, and read as 33 MB instead of 134; training mode stays in float32.  Patches of 256 px and more have more columns than
+        one product may add up in 32 bits: parts of them, each with its own scales, are added in float32.  fc1's module is not called:
+        hooks on it do not fire.  No gradient: call under torch.no_grad()."""
+        weight = self.fc1.weight.detach()
+        K = weight.shape[1]
+        step = K
+        if K > ops.INT8_MAX_K:                                     # equal parts, each a multiple of 128 columns
+            parts = -(-K // (ops.INT8_MAX_K // 128 * 128))
+            step = -(-K // (parts * 128)) * 128
+        columns = [slice(k, k + step) for k in range(0, K, step)]
+        self._int8_fc1, before = [(c,) + tuple(ops.quantize_rows(weight[:, c])) for c in columns], self._int8_fc1
         try:
             yield self
         finally:
@@ -110,8 +118,15 @@ class VGGRegressor(nn.Module):
     def _fc1_relu(self, x):
         if self._int8_fc1 is None or self.training:
             return F.relu(self.fc1(x))
-        w, scale, bias = self._int8_fc1
-        return ops.int8_linear(x, w, scale, bias=bias, relu=True)
+        bias = self.fc1.bias.detach()
+        if len(self._int8_fc1) == 1:
+            _, w, scale = self._int8_fc1[0]
+            return ops.int8_linear(x, w, scale, bias=bias, relu=True)
+        columns, w, scale = self._int8_fc1[0]
+        y = ops.int8_linear(x[:, columns], w, scale, bias=bias)
+        for columns, w, scale in self._int8_fc1[1:]:
+            y += ops.int8_linear(x[:, columns], w, scale)
+        return F.relu_(y)
 
     def forward(self, model_input_nhwc):
         # [B,P,P,2] NHWC -> NCHW-logical view with channels_last strides (no copy)

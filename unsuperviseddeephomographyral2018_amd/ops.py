@@ -760,6 +760,9 @@ def adam_clip_update_(params, grads, exp_avgs, exp_avg_sqs, lr, beta1=0.9, beta2
 
 # ------------------------------------------------------------------------------------------------
 # Products in 8-bit integers (include/uh_model_ops.h through csrc/uhm_torch.cpp): rows of values with one scale each.
+INT8_MAX_K = 131071                 # 131071 * 128^2 < 2^31: the sums of a product stay in 32 bits
+
+
 def quantize_rows(x):
     """Rows of x [..., K] in 8 bits, one scale each -> (q int8 [..., K], scale float32 [...]); q * scale stands for x:
     scale = max |x| / 127 and q = x * (127 / max |x|) rounded to nearest even.  Used for the tokens (rows of activations) and for
@@ -771,7 +774,7 @@ def quantize_rows(x):
 def int8_matmul(x, x_scale, weight, weight_scale, bias=None, relu=False, out_dtype=torch.float32):
     """act((x . weight^T) * x_scale * weight_scale + bias): x int8 [..., K] with one scale per token (x_scale [...]), weight
     int8 [N, K] with one per channel (weight_scale [N]), bias float32 [N] or None, act = relu or nothing -> [..., N] in out_dtype
-    (float32, bfloat16, float16).  The sums are exact (K <= 131071).  No gradient."""
+    (float32, bfloat16, float16).  The sums are exact (K <= INT8_MAX_K = 131071).  No gradient."""
     return _lib.load_torch_ops().int8_matmul(x, x_scale, weight, weight_scale, bias, bool(relu), out_dtype)
 
 
