@@ -16,6 +16,7 @@ import argparse
 import contextlib
 import math
 import os
+import sys
 import time
 
 import numpy as np
@@ -408,8 +409,16 @@ def _ckpt_path(args):
     return d, os.path.join(d, args.model_name + '.pt')
 
 
+def note_shared_devices(rank, world):
+    ranks = int(os.environ.get('LOCAL_WORLD_SIZE', world))
+    if rank == 0 and ranks > 1 and torch.cuda.is_available() and torch.cuda.device_count() < ranks:
+        print('note: %d ranks with %d visible GPU(s): the ranks share the visible device(s) over gloo (a functional run, not a '
+              'scaling run)' % (ranks, torch.cuda.device_count()), file=sys.stderr, flush=True)
+
+
 def train(args):
     rank, world, local = uh_dist.init_from_env()
+    note_shared_devices(rank, world)
     device = torch.device('cuda', local) if torch.cuda.is_available() else None
     if device is None:
         raise RuntimeError('training needs an MI355X: the hot path has no CPU fallback')
@@ -685,7 +694,6 @@ def unsupported_flag_notes(args, argv):
 
 
 def main(argv=None):
-    import sys
     argv = list(sys.argv[1:] if argv is None else argv)
     args = build_parser().parse_args(argv)
     for note in unsupported_flag_notes(args, argv):
@@ -697,9 +705,7 @@ def main(argv=None):
         raise SystemExit('homography_CNN_synthetic: %s' % e)
     if args.mode == 'train':
         if what == 'launch':
-            if 0 < torch.cuda.device_count() < world:     # counting devices does not initialise the GPU: self_launch may still exec
-                print('note: --num_gpus %d with %d visible GPU(s): the ranks share the visible device(s) over gloo (a functional '
-                      'run, not a scaling run)' % (world, torch.cuda.device_count()), file=sys.stderr, flush=True)
+            # no GPU call before this, not even a count of the devices (it may ask the runtime): a process that made one must not exec
             uh_dist.self_launch(world, MODULE, argv, module=True)          # does not return
         train(args)
     else:
