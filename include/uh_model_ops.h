@@ -56,7 +56,8 @@ UHM_API const char* uhm_error_string(int code);
 /* ---- global norm, clipping, clipped Adam -------------------------------------------------------------------------------
  * A list is `count` >= 1 tensors of numel[i] >= 0 contiguous elements of type dtypes[i], each at least element-aligned (16-byte
  * aligned tensors go faster).  numel[i] == 0 tensors are skipped (their pointer may be NULL).  Up to 2^31 - 1 chunks of 4096
- * elements per list.  Sums of squares are held in f64: no finite f32 list over- or underflows.
+ * elements per list.  Sums of squares are held in f64, so that none over- or underflows on the way; the norm is told in f32, and one
+ * above FLT_MAX (100 values of 3e38) is infinite there: it counts as not finite.
  * Workspace: uhm_multi_workspace_bytes(count) bytes, 8-byte aligned.  It overlaps neither the tensors nor a norm of the call.   */
 UHM_API size_t uhm_multi_workspace_bytes(int count);
 
@@ -66,7 +67,7 @@ UHM_API int uhm_global_norm(const void* const* tensors, const long long* numel, 
 
 /* out[i] = tensors[i] * f,  f = clip_norm / n if n > clip_norm, else 1; NaN if n is not finite (as tf.clip_by_global_norm: every
  * value becomes NaN).  n = use_norm[0] when use_norm (a device scalar) is given, else the global norm; norm[0] <- n (norm may
- * be NULL).  out[i] may equal tensors[i] (in place; with f = 1 nothing is then written); any other overlap of an output is
+ * be NULL).  A factor below the normal range of f32 keeps its bits.  out[i] may equal tensors[i] (in place; with f = 1 nothing is then written); any other overlap of an output is
  * UHM_E_OVERLAP, of norm and use_norm too (they may be the same).  0 < clip_norm (may be +inf).  Workspace may be NULL when use_norm
  * is given.                                */
 UHM_API int uhm_clip_by_global_norm(const void* const* tensors, void* const* out, const long long* numel, const int* dtypes,

@@ -11,9 +11,9 @@
 // workspace, and int8_join_kernel adds them (integers: the split does not change the result) and applies the epilogue.
 //
 // Measured on one MI355X (several sets of operands in turn, so that the weight comes from memory; passes among others):
-//   fc1, 1024 x 32768:  1 pair 7.9 us (4.3 TB/s), from float 9.9; 64 pairs 11.0; 128 pairs from float 20.0 (quantising 6, product 11, join 3)
-//   4096 x 4096 x 8192: 134 us with bf16 results; each 8192 of K more take 115 us = 2.4 POP/s.  The loop without loads takes 90 us, with
-//   neither loads nor LDS reads 69 us (the matrix instructions alone, at the clock that their power leaves): power, not latency.
+//   fc1, 1024 x 32768:  1 pair 7.9 us (4.2 TB/s), from float 9.8; 64 pairs 11.2; 128 pairs from float 21.5 (quantising 6, product 11, join 3)
+//   4096 x 4096 x 8192: 134 - 143 us with bf16 results, by card.  Where it takes 134, each 8192 of K more take 115 us = 2.4 POP/s; the loop without loads
+//   takes 90 us, with neither loads nor LDS reads 69 us (the matrix instructions alone, at the clock that their power leaves): power, not latency.
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -491,18 +491,19 @@ __global__ __launch_bounds__(T) void int8_few_kernel(const void* __restrict__ x,
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 constexpr long long MAX_K = 131071, MAX_DIM = 0x7fffffffLL - 512;
 constexpr long long MAX_LD = 1LL << 23;     // 256 rows of it are indexed in 32 bits
-constexpr long long FEW = 2;               // tokens up to which int8_few_kernel reads the weight (fc1: 2 tokens 10.7 us, 4 12.5; tiles, 8 tokens, 12.2)
+constexpr long long FEW = 2;               // tokens up to which int8_few_kernel reads the weight (fc1, replayed: 2 tokens 10.7 us, 4 12.5; tiles 12.2)
 
 struct Plan { int bm, bn, splits, tiles_per_split; };
 
-// The tile by how many of them there are, splits of K where they do not fill the 256 CUs (each measured against every other tile and
-// split on 16 shapes; the rule is within 8 % of the best of each).  us, tile / splits taken | the other side:
-//   32 x 128 up to 32 tokens:  16 x 1024 x 32768 12.2 at 32 splits | 13.8 at 64
-//   256 x 256 from 200 tiles:  4096 x 4096 x 8192 154 | 210 with 128 x 128; below, 1500 x 1500 x 3000 (36 of them) 27 | 56
-//   128 x 128 from 200 tiles:  2048 x 2048 x 2048 23.2 | 24.5 with 64 x 64; below, 1024 x 1024 x 1024 (64 of them) 8.7 | 15.9
-//   64 x 64:                   64 x 1024 x 32768 13.1 at 16 splits | 14.2 at 32, 15.7 at 8; 1000 x 300 x 6000 14.3 at 4 | 17.3 at 8, 18.9 at 1
+// The tile by how many of them there are, splits of K where they do not fill the 256 CUs.  Measured against the other tiles and splits on 19
+// shapes, f32 results, replays of captured calls (about 1 us a launch more than passes among others): within 7 % of the best of each but for
+// 128 x 1024 x 32768, 19.1 us at 16 splits | 16.7 at 8.  us, tile / splits taken | the other side:
+//   32 x 128 up to 32 tokens:  16 x 1024 x 32768 12.5 at 32 splits | 12.3 at 16, 14.2 at 64
+//   256 x 256 from 200 tiles:  4096 x 4096 x 8192 151 | 207 with 128 x 128; below, 1500 x 1500 x 3000 (36 of them) 27.5 | 56.5
+//   128 x 128 from 200 tiles:  2048 x 2048 x 2048 23.6 | 27.1 with 64 x 64; below, 1024 x 1024 x 1024 (64 of them) 8.9 | 15.9
+//   64 x 64:                   64 x 1024 x 32768 13.1 at 16 splits | 14.6 at 32, 15.7 at 8; 1000 x 300 x 6000 14.7 at 5 | 14.4 at 4, 17.5 at 8, 19.0 at 1
 // At least 8 tiles of K per split (a block's first loads take as long as several tiles), 4 where there are few blocks anyway:
-// 100 x 50 x 5000 7.8 | 8.8.
+// 100 x 50 x 5000 8.2 at 10 | 7.9 at 16.
 inline Plan plan_of(long long M, long long N, long long K) {
     const auto tiles_of = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
     Plan p;

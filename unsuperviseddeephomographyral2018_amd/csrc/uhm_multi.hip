@@ -14,7 +14,7 @@
 // b + 2 grid, ... of the concatenated chunk list, a fixed assignment, so that sums do not depend on timing.
 // f64 sums: squares of f32 neither overflow (|t| up to 3e38) nor vanish (down to 1e-45), and the kernel stays memory-bound
 // (one f64 FMA per element at half the f32 rate).
-// One MI355X, us a pass: norm of the 128 px regressor's gradients (137 MB) 28.6, of 300 small tensors 17; clipping 71.0 / 40 small ones
+// One MI355X, us a pass: norm of the 128 px regressor's gradients (137 MB) 28.5, of 300 small tensors 18; clipping 70.7 / 40 small ones
 // 18; Adam with clipping 182 (957 MB without the second read of the gradients: 5.3 TB/s), at 32 px (77 MB) 19.
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>

@@ -726,7 +726,8 @@ def conv_bias_relu_pool(x, weight, bias, padding=1):
 def global_norm(tensors):
     """sqrt of the sum of all squares over a list of float32 / bfloat16 / float16 tensors (mixed, of any shapes and dense or
     strided layouts, empty ones among them), as tf.global_norm -> float32 scalar on their device.  Squares are added in f64 in a
-    fixed order: the result is the same on every call, and finite lists neither overflow nor vanish on the way.  No gradient."""
+    fixed order: the result is the same on every call, and finite lists neither overflow nor vanish on the way (a norm past the range
+    of float32 itself is inf).  No gradient."""
     return _lib.load_torch_ops().global_norm(tensors)
 
 
@@ -774,12 +775,15 @@ def quantize_rows(x):
 def int8_matmul(x, x_scale, weight, weight_scale, bias=None, relu=False, out_dtype=torch.float32):
     """act((x . weight^T) * x_scale * weight_scale + bias): x int8 [..., K] with one scale per token (x_scale [...]), weight
     int8 [N, K] with one per channel (weight_scale [N]), bias float32 [N] or None, act = relu or nothing -> [..., N] in out_dtype
-    (float32, bfloat16, float16).  The sums are exact (K <= INT8_MAX_K = 131071).  No gradient."""
+    (float32, bfloat16, float16).  The sums are exact (K <= INT8_MAX_K = 131071).  Rows laid out as quantize_rows lays them out (16-byte
+    aligned, a multiple of 16 bytes apart) are read in place; others, contiguous ones whose K is no multiple of 16 among them, are
+    copied on every call: a weight that is used again is better kept as quantize_rows gives it.  No gradient."""
     return _lib.load_torch_ops().int8_matmul(x, x_scale, weight, weight_scale, bias, bool(relu), out_dtype)
 
 
 def int8_linear(x, weight, weight_scale, bias=None, relu=False):
     """A fully connected layer in 8-bit integers: the rows of x (float32 / bfloat16 / float16 [..., K]) are quantised on the way
     (quantize_rows) and multiplied with a weight that was quantised before (weight, weight_scale = quantize_rows(W), W [N, K])
-    -> act(x . W^T + bias) [..., N] in x's type.  Evaluation only: no gradient."""
+    -> act(x . W^T + bias) [..., N] in x's type.  The weight is read in place where int8_matmul reads its rows in place.  Evaluation
+    only: no gradient."""
     return _lib.load_torch_ops().int8_linear(x, weight, weight_scale, bias, bool(relu))
