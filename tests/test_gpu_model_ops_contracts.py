@@ -119,6 +119,30 @@ def test_views_that_interleave_are_clipped(ops, dev, make):
         assert torch.equal(big[~inside], kept[~inside])
 
 
+def test_memory_that_a_copy_stands_for_is_compared_too(ops, dev, UHError):
+    """A norm inside a view that is clipped in a copy; gradients in another order than their variable, over variables and moments."""
+    big = torch.ones(12, 12, device=dev)
+    for norm in (big[3, 2], big[0, 0], big[11, 2]):
+        with pytest.raises(UHError, match='twice'):
+            ops.clip_by_global_norm_([big[:, :3]], 1.0, use_norm=norm)
+    assert bool((big == 1).all())
+    ops.clip_by_global_norm_([big[:, :3]], 0.5, use_norm=big[4, 3])          # beside it
+    assert bool((big[:, :3] == 0.5).all()) and bool((big[:, 3:] == 1).all())
+
+    make = lambda: [torch.ones(6, 6, device=dev) for _ in range(4)]
+    for k in range(3):
+        p, m, v, other = make()
+        g = (p, m, v)[k].t()
+        with pytest.raises(UHError, match='shares elements'):
+            ops.adam_clip_update_([other, p], [other.clone(), g], [torch.zeros_like(other), m], [torch.zeros_like(other), v], lr=1e-2)
+        assert all(bool((t == 1).all()) and t._version == 0 for t in (p, m, v, other))
+    p, m, v, g = make()
+    wide = torch.ones(6, 13, device=dev)                                    # beside, within the same rows
+    ops.adam_clip_update_([p], [wide[:, 1:7].t()], [m], [v], lr=1e-2)
+    ops.adam_clip_update_([p], [g[:1].expand(6, 6)], [m], [v], lr=1e-2)     # gradients may repeat themselves: they are read
+    ops.adam_clip_update_([p, p.clone()], [g.t(), g.t()], [m, m.clone()], [v, v.clone()], lr=1e-2)
+
+
 # ---- the ends of f32 ------------------------------------------------------------------------------------------------------------
 FAR = [(1e37, 1e-3), (1e37, 3.9), (1e30, 1e-37), (1e36, 1e-10), (1e37, 2.0 ** -149), (1.0, 1e-40)]
 

@@ -296,7 +296,7 @@ struct View {
         : base((uintptr_t)v.data_ptr()), end(base + v.element_size()), width(v.element_size()), copied(v.is_neg() || !v.is_non_overlapping_and_dense()) {
         for (int64_t i = 0; i < v.dim(); ++i) {
             const int64_t stride = v.stride(i) * width, last = v.size(i) - 1;
-            if (last < 1) continue;
+            if (last < 1 || stride == 0) continue;                      // (an expanded dimension adds no bytes)
             dims.push_back({stride, last});
             end += stride * last;
             if (stride > row) { row = stride; rows = stride * last; }
@@ -304,6 +304,7 @@ struct View {
         within = (int64_t)(end - base) - rows;
     }
     bool shares(const View& o) const {
+        if (base >= o.end || o.base >= end) return false;
         const int64_t gap = (int64_t)(o.base - base);
         if (row && row == o.row && gap >= 0 && gap % row >= within && gap % row + o.within <= row) return false;      // other columns of the same rows
         Terms terms;
@@ -321,7 +322,7 @@ struct View {
     }
 };
 
-// whether an element of a view that is clipped in a copy is given twice (among tensors without gaps the native call checks that)
+// whether memory of a view that is clipped in a copy is given twice (among tensors without gaps the native call checks that)
 bool shares_elements(const vector<const Tensor*>& ts) {
     if (std::none_of(ts.begin(), ts.end(), [](const Tensor* t) { return t->is_neg() || !t->is_non_overlapping_and_dense(); })) return false;
     vector<View> v;
@@ -348,7 +349,9 @@ Tensor clip_by_global_norm_(const py::object& tensors, double clip_norm, const p
         for (int64_t i = 0; i < t->dim() && t->numel(); ++i)            // slices of something larger: clipped in a copy
             if (t->stride(i) == 0 && t->size(i) > 1) fail(string(name) + ": an expanded tensor cannot be written in place");
     }
-    if (shares_elements(given)) fail(string(name) + ": the same elements are given twice (views that overlap)");
+    vector<const Tensor*> memory = given;
+    if (use_norm.defined()) memory.push_back(&use_norm);
+    if (shares_elements(memory)) fail(string(name) + ": the same elements are given twice (views that overlap)");
     const Call call(l.device);
     l.make_dense();
     const Tensor norm = clip(call, Described(l), pointers(l), clip_norm, use_norm, name);
@@ -380,6 +383,7 @@ Tensor adam_clip_update_(const py::object& params, const py::object& grads, cons
     if (g.device != p.device || m.device != p.device || v.device != p.device) fail(string(name) + ": lists on several devices");
     const Tensor use_norm = given_norm(use, p.device, name);
     const Call call(p.device);
+    vector<size_t> reordered;                                          // gradients that a copy takes the place of
     for (size_t i = 0; i < n; ++i) {
         const Tensor &pi = *p.t[i], &gi = *g.t[i], &mi = *m.t[i], &vi = *v.t[i];
         no_gradient_but_of_leaves(pi, name);
@@ -388,12 +392,19 @@ Tensor adam_clip_update_(const py::object& params, const py::object& grads, cons
             fail(string(name) + ": shapes " + shape_of(pi) + ", " + shape_of(gi) + ", " + shape_of(mi) + ", " + shape_of(vi));
         if (!pi.is_non_overlapping_and_dense() || !laid_out_alike(pi, mi) || !laid_out_alike(pi, vi) || pi.is_neg() || mi.is_neg() || vi.is_neg())
             fail(string(name) + ": params and moments must be dense and laid out alike");
-        if (gi.is_neg() || !laid_out_alike(pi, gi)) {                  // a gradient in another order
-            Tensor same = at::empty_strided(pi.sizes(), pi.strides(), gi.options().requires_grad(false));
-            at::NoGradGuard no_grad;
-            same.copy_(gi);
-            g.replace(i, same);
-        }
+        if (gi.is_neg() || !laid_out_alike(pi, gi)) reordered.push_back(i);
+    }
+    for (size_t i : reordered) {                                       // the native check sees the copies
+        const View gi(*g.t[i]);
+        for (const List* l : {&p, &m, &v})
+            for (const Tensor* t : l->t)
+                if (g.t[i]->numel() && t->numel() && gi.shares(View(*t))) fail(string(name) + ": a gradient shares elements with params or moments");
+    }
+    for (size_t i : reordered) {                                       // a gradient in another order
+        Tensor same = at::empty_strided(p.t[i]->sizes(), p.t[i]->strides(), g.t[i]->options().requires_grad(false));
+        at::NoGradGuard no_grad;
+        same.copy_(*g.t[i]);
+        g.replace(i, same);
     }
     const Described d(g);
     vector<const void*> pp = pointers(p), pm = pointers(m), pv = pointers(v);
